@@ -175,7 +175,8 @@ def _verify_data(case, seed):
     at = torch.rand(b, n, 1, generator=g, device="cuda")
     tokens = (probs.double().cumsum(-1) <= at).sum(-1).clamp(max=vocab - 1).to(torch.int32)
     return dict(target=target.contiguous(), draft=draft.contiguous() if case["draft_model"] else None, tokens=tokens,
-                uniforms=torch.rand(b, n + 1, generator=g, device="cuda"), temperature=0.8)
+                uniforms=torch.rand(b, n + 1, generator=g, device="cuda"),
+                temperature=torch.tensor(0.8).item())   # the 32-bit number that an option holds
 
 
 _shared = {}
