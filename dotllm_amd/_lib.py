@@ -68,6 +68,25 @@ class Sampling(C.Structure):
                 ("repeat_penalty", C.c_float), ("repeat_window", C.c_int32)]
 
 
+class KvCacheDesc(C.Structure):
+    """llmdot_hip_kv_cache_desc (include/llmdot_hip_cache.h)."""
+    _fields_ = [("slots", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("capacity", C.c_int32),
+                ("k_type", C.c_uint32), ("v_type", C.c_uint32)]
+
+
+class TokenBatch(C.Structure):
+    """llmdot_hip_token_batch: device addresses of slots, starts and counts."""
+    _fields_ = [("batch", C.c_int32), ("tokens", C.c_int32), ("slots", C.c_void_p), ("starts", C.c_void_p),
+                ("counts", C.c_void_p)]
+
+
+class Attention(C.Structure):
+    """llmdot_hip_attention."""
+    _fields_ = [("heads", C.c_int32), ("window", C.c_int32), ("scale", C.c_float), ("prefix", C.c_void_p),
+                ("prefix_slot", C.c_int32), ("prefix_len", C.c_int32), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64)]
+
+
 class StepTiming(C.Structure):
     _fields_ = [("total_ms", C.c_float), ("gemv_ms", C.c_float), ("gemv_launches", C.c_int32),
                 ("gemv_bytes", C.c_double)]
@@ -137,6 +156,19 @@ SIGNATURES = {
     "llmdot_hip_synth_weights": [_U32, _I64, _I64, _U64, _F, _P, _I32],
 }
 
+# The operators over device memory (include/llmdot_hip_cache.h).
+CACHE_SIGNATURES = {
+    "llmdot_hip_stream": [_P, _PP],
+    "llmdot_hip_kv_cache_create": [_P, C.POINTER(KvCacheDesc), _PP],
+    "llmdot_hip_kv_cache_destroy": [_P],
+    "llmdot_hip_kv_cache_write": [_P, _P, _I64, _P, _I64, C.POINTER(TokenBatch)],
+    "llmdot_hip_kv_cache_read": [_P, _P, _I64, _P, _I64, C.POINTER(TokenBatch)],
+    "llmdot_hip_kv_cache_attention": [_P, _P, _P, C.POINTER(TokenBatch), C.POINTER(Attention), _P, C.c_size_t],
+    "llmdot_hip_kv_cache_attention_workspace": [_P, _I32, _I32, _I32, _I32, C.POINTER(C.c_size_t)],
+    "llmdot_hip_verify_drafts": [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _F, _P, _P, _P, C.c_size_t],
+    "llmdot_hip_verify_drafts_workspace": [_P, _I32, _I32, _I32, C.POINTER(C.c_size_t)],
+}
+
 _lib = None
 _lock = threading.Lock()
 
@@ -150,7 +182,7 @@ def lib() -> C.CDLL:
         if not os.path.exists(LIB_PATH):
             raise ImportError(f"{LIB_PATH} is missing: build it with dotllm_amd.build.build()")
         handle = C.CDLL(LIB_PATH)
-        for name, argtypes in SIGNATURES.items():
+        for name, argtypes in {**SIGNATURES, **CACHE_SIGNATURES}.items():
             fn = getattr(handle, name)
             fn.argtypes = argtypes
             fn.restype = C.c_int32

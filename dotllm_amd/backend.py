@@ -206,6 +206,48 @@ class HipBackend:
                                       C.byref(tok)))
         return tok.value
 
+    # -- operators over device memory (include/llmdot_hip_cache.h; no counterpart
+    #    in the reference) ---------------------------------------------------------
+    @property
+    def stream(self) -> int:
+        """The hipStream_t every call of this backend runs on (torch.cuda.ExternalStream takes it)."""
+        p = C.c_void_p()
+        _call(lib().llmdot_hip_stream(self._ctx, C.byref(p)))
+        return p.value
+
+    def synchronize(self) -> None:
+        _call(lib().llmdot_hip_synchronize(self._ctx))
+
+    def verify_workspace(self, batch: int, drafts: int, vocab: int):
+        """Device memory that suffices for verify_drafts calls of that size."""
+        from .device import DeviceArray
+        n = C.c_size_t(0)
+        _call(lib().llmdot_hip_verify_drafts_workspace(self._ctx, batch, drafts, vocab, C.byref(n)))
+        return DeviceArray(self, (n.value,), "uint8")
+
+    def verify_drafts(self, target, drafts, uniforms, tokens_out, accepted_out, *, temperature: float, workspace,
+                      draft=None, counts=None) -> None:
+        """Speculative sampling on the device: which drafted tokens stand against the target
+        model's logits, and the token that follows them.  target [batch, n + 1, vocab] float32,
+        drafts [batch, n] int32, uniforms [batch, n + 1] float32 (the draws that decide each draft,
+        then the one for the next token), draft [batch, n, vocab] the draft model's logits (None:
+        drafts that came with certainty), counts [batch] int32 (None: n each).  tokens_out
+        [batch, n + 1]: the standing drafts, the next token, then -1; accepted_out [batch]: how
+        many stand.  All arrays in device memory; temperature <= 0 is greedy."""
+        from .device import address
+        dev = self.device
+        b, n1, vocab = target.shape
+        n = n1 - 1
+        tp = address(target, "target", "float32", (b, n1, vocab), dev)
+        dp = address(drafts, "drafts", "int32", (b, n), dev)
+        up = address(uniforms, "uniforms", "float32", (b, n1), dev)
+        op = address(tokens_out, "tokens_out", "int32", (b, n1), dev)
+        ap = address(accepted_out, "accepted_out", "int32", (b,), dev)
+        qp = address(draft, "draft", "float32", (b, n, vocab), dev) if draft is not None else None
+        cp = address(counts, "counts", "int32", (b,), dev) if counts is not None else None
+        _call(lib().llmdot_hip_verify_drafts(self._ctx, tp, qp, dp, cp, up, b, n, vocab, temperature, op, ap,
+                                             workspace.data_ptr(), workspace.nbytes))
+
     # Members the LLaMA-like decode path does not call (other templates), on
     # the device like the rest (ICB:12, 18, 19, 25, 26).
     def layer_norm(self, inp, weights, bias, output, epsilon: float) -> None:

@@ -31,6 +31,7 @@
 
 #include "../../include/llmdot_hip.h"
 #include "common.h"
+#include "context.h"
 #include "kernels.h"
 
 using namespace llmdot;
@@ -112,8 +113,8 @@ struct llmdot_hip_ctx {
     uint8_t* bounce = nullptr;
     size_t bounce_used = 0;
     hipEvent_t fork = nullptr, join[2] = {nullptr, nullptr};
-    // models created on this context and not yet destroyed; llmdot_hip_destroy
-    // with models alive defers the release to the last model's destroy
+    // models and KV caches created on this context and not yet destroyed;
+    // llmdot_hip_destroy with some alive defers the release to the last one's destroy
     int models = 0;
     bool closing = false;
     // fp32 copies models keep of non-F32 norm weights (LM:63-75): an in-place
@@ -355,6 +356,18 @@ extern "C" int32_t llmdot_hip_destroy(llmdot_hip_ctx* ctx) {
     }
     ctx_release(ctx);
     return 0;
+}
+
+int llmdot::ctx_fail(int code, const std::string& msg) { return fail(code, msg); }
+int llmdot::ctx_device(const llmdot_hip_ctx* ctx) { return ctx->device; }
+hipStream_t llmdot::ctx_stream(const llmdot_hip_ctx* ctx) { return ctx->stream; }
+bool llmdot::ctx_hold(llmdot_hip_ctx* ctx) {
+    if (ctx->closing) return false;
+    ctx->models++;
+    return true;
+}
+void llmdot::ctx_drop(llmdot_hip_ctx* ctx) {
+    if (--ctx->models == 0 && ctx->closing) ctx_release(ctx);
 }
 
 extern "C" int32_t llmdot_hip_get_device_info(llmdot_hip_ctx* ctx, llmdot_hip_device_info* out) {
@@ -1382,7 +1395,7 @@ extern "C" int32_t llmdot_hip_model_destroy(llmdot_hip_model* m) {
         if (it != ctx->weights.end()) it->second.pins--;
     }
     delete m;
-    if (--ctx->models == 0 && ctx->closing) ctx_release(ctx);
+    ctx_drop(ctx);
     return 0;
 }
 

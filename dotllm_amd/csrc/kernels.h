@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kv_layout.h"
+
 namespace llmdot {
 
 // ---- dequant.hip ----
@@ -298,5 +300,39 @@ hipError_t launch_prefill_attn_wave(const PfAttnArgs& a, hipStream_t s);
 // Embedding rows tokens[0..T) (device ids) into out[T][hidden].
 hipError_t launch_embed_rows(const uint8_t* table, uint32_t type, int hidden, const int32_t* tokens, int T, float* out,
                              hipStream_t s);
+
+// ---- kv_cache.hip, kv_attention.hip (quantised KV cache) ----
+// Rows of k and v [batch * tokens], ks and vs floats apart, into the cache, and back.
+hipError_t launch_kv_write(const KvView& c, const KvRows& rows, const float* k, int64_t ks, const float* v, int64_t vs,
+                           hipStream_t s);
+hipError_t launch_kv_read(const KvView& c, const KvRows& rows, float* k, int64_t ks, float* v, int64_t vs,
+                          hipStream_t s);
+struct KvAttnArgs {
+    KvView cache, prefix;     // prefix: read where prefix_len > 0
+    KvRows rows;
+    const float* q;           // [batch * tokens][heads * head_dim], q_stride floats apart
+    float* out;
+    int64_t q_stride, out_stride;
+    int heads, window;
+    int prefix_slot, prefix_len;
+    float scale;
+    uint8_t* work;            // kv_attention_workspace bytes
+};
+bool kv_attention_supported(int head_dim);
+size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix);
+hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s);
+
+// ---- verify.hip (verification of drafted tokens) ----
+struct VerifyArgs {
+    const float *target, *draft;    // [batch][drafts + 1][vocab], [batch][drafts][vocab] or null
+    const int32_t *draft_tokens, *counts;
+    const float* uniforms;          // [batch][drafts + 1]
+    int batch, drafts, vocab;
+    float temperature;
+    int32_t *tokens_out, *accepted_out;
+    uint8_t* work;                  // verify_workspace bytes
+};
+size_t verify_workspace(int batch, int drafts, int vocab);
+hipError_t launch_verify(const VerifyArgs& a, hipStream_t s);
 
 }  // namespace llmdot

@@ -1,0 +1,81 @@
+// kv_layout.h -- where the quantised KV cache keeps its values.
+//
+// A kv head of a slot is a run of records of 32 positions, K and V apart:
+//   [head_dim / 32 blocks][64 lanes]  integers, 16 bytes a lane (Q8_0) or 8 (Q4_0)
+//   [head_dim / 32 blocks][32]        fp16 scales, one per position
+//   V only: [32]                      fp16 exponent: 2^e > the position's largest |scale| >= 2^(e-1)
+// so that one 16-byte load per lane is an operand of v_mfma_f32_16x16x32_f16
+// once its bytes are halves, without LDS or lane exchanges: lane (g, c) = (lane
+// >> 4, lane & 15) of a block holds
+//   K  dims 8 g .. 8 g + 7 of positions c and 16 + c (A operands of K q^T, one
+//      MFMA per 16 positions and block of 32 dims: a scale never changes inside
+//      one product),
+//   V  dims c and 16 + c of positions 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3,
+//      which are the rows that lane (g, .) holds of two such score tiles: the
+//      probabilities are the B operand of V^T p^T where they stand.
+// Scales and exponents are ordered by those rows too: position p at 8 g + j.
+// Q8_0 integers are stored as q + 128, Q4_0 as q + 8: a byte b becomes the half
+// 1024 + b by setting its high byte to 0x64, and one packed add takes 1024 and
+// the offset off again.
+#pragma once
+
+#include "common.h"
+
+namespace llmdot {
+
+constexpr int KV_GROUP = 32;   // positions per record
+
+__host__ __device__ constexpr int kv_block_bytes(bool q4) { return q4 ? 512 : 1024; }
+__host__ __device__ constexpr int kv_record_bytes(bool q4, int blocks, bool v) {
+    return blocks * (kv_block_bytes(q4) + 64) + (v ? 64 : 0);
+}
+
+// Order of a position within its record's scales.
+__host__ __device__ constexpr int kv_row(int p) { return (p & 12) * 2 + (p & 3) + (p >> 4) * 4; }
+
+// Byte of element (position p of the record, dim r of its block); Q4_0: the
+// nibble is kv_k_high / kv_v_high.
+__host__ __device__ constexpr int kv_k_byte(bool q4, int p, int r) {
+    const int lane = (r >> 3) * 16 + (p & 15), t = p >> 4;
+    return q4 ? lane * 8 + t * 4 + (r & 3) : lane * 16 + t * 8 + (r & 7);
+}
+__host__ __device__ constexpr int kv_k_high(int r) { return (r >> 2) & 1; }
+__host__ __device__ constexpr int kv_v_byte(bool q4, int p, int r) {
+    const int lane = ((p >> 2) & 3) * 16 + (r & 15), j = (p & 3) + (p >> 4) * 4;
+    return q4 ? lane * 8 + j : lane * 16 + (r >> 4) * 8 + j;
+}
+__host__ __device__ constexpr int kv_v_high(int r) { return r >> 4; }
+
+struct KvView {
+    uint8_t *k, *v;             // [slots][kv_heads][groups] records
+    int slots, kv_heads, head_dim, capacity, groups;
+    int k_q4, v_q4;
+    int k_rec, v_rec;           // bytes of a record
+};
+__host__ __device__ inline int64_t kv_group_index(const KvView& c, int slot, int head, int group) {
+    return ((int64_t)slot * c.kv_heads + head) * c.groups + group;
+}
+
+struct KvRows {                 // llmdot_hip_token_batch
+    int batch, tokens;
+    const int32_t *slots, *starts, *counts;
+};
+// Sequence b's tokens as the kernels see them: rows lo .. hi - 1 of the call are
+// positions start + lo .. start + hi - 1, all inside the slot (lo = hi: none).
+struct KvSpan {
+    int slot, start, lo, hi;
+};
+__device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, int b) {
+    KvSpan s{r.slots[b], r.starts[b], 0, r.counts ? r.counts[b] : r.tokens};
+    if (s.hi > r.tokens) s.hi = r.tokens;
+    if (s.slot < 0 || s.slot >= c.slots || s.hi <= 0 || s.start >= c.capacity || s.start <= -r.tokens) {
+        s.slot = s.start = s.hi = 0;
+        return s;
+    }
+    if (s.start < 0) s.lo = -s.start;
+    if (s.hi > c.capacity - s.start) s.hi = c.capacity - s.start;   // start > -2^31 here: no overflow
+    if (s.hi < s.lo) s.hi = s.lo;
+    return s;
+}
+
+}  // namespace llmdot
