@@ -1,78 +1,650 @@
 // kv_attention.hip -- attention over the quantised KV cache (layout: kv_layout.h).
+//
+// out = sum_t softmax_t(scale q . k_t) v_t with k_t = dk qk, v_t = dv qv: integers
+// times a scale per position and block of 32 dims.  One pass over the keys with
+// the running maximum and sum, on v_mfma_f32_16x16x32_f16:
+//   scores  S^T = K q^T: one MFMA covers exactly one block, so K's integers are
+//     exact operands and its scale multiplies the MFMA's result (one FMA per
+//     block and score).  q enters as two halves (22 bits), scaled by a power of
+//     two per row.
+//   values  O^T += V^T P'^T with P' = p dv, the probability with V's scale on it,
+//     again two halves, per block; the score tile's lanes hold P' where the MFMA
+//     wants it.  The running reference is the maximum of s + e, 2^e past the
+//     position's largest |dv|: then p 2^e <= 2^14 and P' <= 2^14 whatever V's
+//     range, so halves neither overflow nor lose small values.  p 2^e = ph + pl
+//     and dv 2^-e are halves, and ph dvn = hi + r exactly (r an fma), so
+//     P' = hi + (pl dvn + r) costs three packed instructions for two values.
+// Scores, statistics and sums are fp32.
 #include "kernels.h"
 #include "kv_layout.h"
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace llmdot {
 
 namespace {
 
-__device__ __forceinline__ float kv_k_value(const KvView& c, const uint8_t* rec, int p, int d) {
-    const int blocks = c.head_dim / 32, blk = d >> 5, r = d & 31;
-    uint32_t u = rec[blk * kv_block_bytes(c.k_q4) + kv_k_byte(c.k_q4, p, r)];
-    if (c.k_q4) u = (kv_k_high(r) ? u >> 4 : u) & 15;
-    const float s = (float)*reinterpret_cast<const _Float16*>(rec + blocks * kv_block_bytes(c.k_q4) + blk * 64 + kv_row(p) * 2);
-    return s * (float)((int)u - (c.k_q4 ? 8 : 128));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int THREADS = 256, WAVES = 4;
+constexpr float P_EXP = 14.f;   // probabilities are held times 2^14
+
+// ---- operands ----
+// Bytes b of w (unsigned, off more than the integer) as halves: 0x6400 + b is 1024 + b.
+__device__ __forceinline__ h2 byte_halves(uint32_t w, uint32_t sel, _Float16 off) {
+    const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w, sel);
+    return __builtin_bit_cast(h2, x) - h2{off, off};
 }
-__device__ __forceinline__ float kv_v_value(const KvView& c, const uint8_t* rec, int p, int d) {
-    const int blocks = c.head_dim / 32, blk = d >> 5, r = d & 31;
-    uint32_t u = rec[blk * kv_block_bytes(c.v_q4) + kv_v_byte(c.v_q4, p, r)];
-    if (c.v_q4) u = (kv_v_high(r) ? u >> 4 : u) & 15;
-    const float s = (float)*reinterpret_cast<const _Float16*>(rec + blocks * kv_block_bytes(c.v_q4) + blk * 64 + kv_row(p) * 2);
-    return s * (float)((int)u - (c.v_q4 ? 8 : 128));
+__device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
+    return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+constexpr uint32_t LOW_PAIR = 0x04010400u, HIGH_PAIR = 0x04030402u;
+
+// A lane's 16 integers of a block: operands for (K) positions c and 16 + c, (V) dims c and 16 + c.
+template <bool Q4>
+struct Ints {
+    typename std::conditional<Q4, u2, u4>::type w;
+    __device__ __forceinline__ void load(const uint8_t* block, int lane) {
+        w = *reinterpret_cast<const decltype(w)*>(block + lane * sizeof(w));
+    }
+    // K: each half of the lane's bytes is one operand (Q4_0: low nibbles are dims 0 .. 3, high 4 .. 7)
+    __device__ __forceinline__ h8 k(int t) const {
+        if constexpr (Q4) {
+            const uint32_t lo = w[t] & 0x0F0F0F0Fu, hi = (w[t] >> 4) & 0x0F0F0F0Fu;
+            const _Float16 off = (_Float16)1032.f;
+            return join(byte_halves(lo, LOW_PAIR, off), byte_halves(lo, HIGH_PAIR, off), byte_halves(hi, LOW_PAIR, off),
+                        byte_halves(hi, HIGH_PAIR, off));
+        } else {
+            const _Float16 off = (_Float16)1152.f;
+            return join(byte_halves(w[2 * t], LOW_PAIR, off), byte_halves(w[2 * t], HIGH_PAIR, off),
+                        byte_halves(w[2 * t + 1], LOW_PAIR, off), byte_halves(w[2 * t + 1], HIGH_PAIR, off));
+        }
+    }
+    // V: Q4_0 keeps dims c in the low nibbles and 16 + c in the high ones
+    __device__ __forceinline__ h8 v(int t) const {
+        if constexpr (Q4) {
+            const uint32_t a = (w[0] >> (4 * t)) & 0x0F0F0F0Fu, b = (w[1] >> (4 * t)) & 0x0F0F0F0Fu;
+            const _Float16 off = (_Float16)1032.f;
+            return join(byte_halves(a, LOW_PAIR, off), byte_halves(a, HIGH_PAIR, off), byte_halves(b, LOW_PAIR, off),
+                        byte_halves(b, HIGH_PAIR, off));
+        } else {
+            return k(t);
+        }
+    }
+};
+
+// Eight fp32 values as two planes of halves.
+__device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const h2 h = __builtin_convertvector(f2{x[i], x[i + 1]}, h2);
+        const h2 l = __builtin_convertvector(f2{x[i] - (float)h[0], x[i + 1] - (float)h[1]}, h2);
+        hi[i] = h[0]; hi[i + 1] = h[1];
+        lo[i] = l[0]; lo[i + 1] = l[1];
+    }
 }
 
-// One wavefront per query head of a token: 64 keys at a time, one per lane,
-// with the running maximum and sum; then the lanes take the dims.
-__global__ __launch_bounds__(64) void kv_attention_simple(KvAttnArgs a) {
-    const KvView& c = a.cache;
-    const int h = blockIdx.x % a.heads, rest = blockIdx.x / a.heads;
-    const int i = rest % a.rows.tokens, b = rest / a.rows.tokens;
-    const KvSpan sp = kv_span(a.rows, c, b);
-    if (i < sp.lo || i >= sp.hi) return;
-    const int hd = c.head_dim, lane = threadIdx.x, head = h / (a.heads / c.kv_heads);
-    const int64_t row = (int64_t)b * a.rows.tokens + i;
-    const float* q = a.q + row * a.q_stride + h * hd;
-    __shared__ float qs[256], ps[64];
-    for (int d = lane; d < hd; d += 64) qs[d] = q[d] * a.scale;
-    __syncthreads();
-    const int P = a.prefix_len;
-    const int64_t end = (int64_t)P + sp.start + i + 1;
-    const int64_t begin = a.window > 0 && end > a.window ? end - a.window : 0;
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t t0 = begin; t0 < end; t0 += 64) {
-        const int64_t t = t0 + lane;
-        float s = -INFINITY;
-        if (t < end) {
-            const bool pre = t < P;
-            const KvView& w = pre ? a.prefix : c;
-            const int p = (int)(pre ? t : t - P);
-            const uint8_t* rec = w.k + kv_group_index(w, pre ? a.prefix_slot : sp.slot, head, p / KV_GROUP) * w.k_rec;
-            s = 0.f;
-            for (int d = 0; d < hd; d++) s = fmaf(qs[d], kv_k_value(w, rec, p % KV_GROUP, d), s);
+// One record's K or V of a block set, in registers.
+template <bool Q4, int NB>
+struct Record {
+    Ints<Q4> q[NB];
+    h8 d[NB];          // scales of the lane's positions
+    __device__ __forceinline__ void load(const uint8_t* rec, int lane) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            q[i].load(rec + i * kv_block_bytes(Q4), lane);
+            d[i] = *reinterpret_cast<const h8*>(rec + NB * kv_block_bytes(Q4) + i * 64 + (lane >> 4) * 16);
         }
-        const float mn = fmaxf(m, wave_max(s));
-        const float p = t < end ? expf(s - mn) : 0.f;
-        const float f = m == -INFINITY ? 0.f : expf(m - mn);
-        l = l * f + wave_sum(p);
-        m = mn;
-        ps[lane] = p;
-        __syncthreads();
-        for (int x = 0; x < 4; x++) acc[x] *= f;
-        for (int j = 0; j < 64 && t0 + j < end; j++) {
-            const int64_t u = t0 + j;
-            const bool pre = u < P;
-            const KvView& w = pre ? a.prefix : c;
-            const int pp = (int)(pre ? u : u - P);
-            const uint8_t* rec = w.v + kv_group_index(w, pre ? a.prefix_slot : sp.slot, head, pp / KV_GROUP) * w.v_rec;
-            for (int x = 0; x < 4 && x * 64 + lane < hd; x++)
-                acc[x] = fmaf(ps[j], kv_v_value(w, rec, pp % KV_GROUP, x * 64 + lane), acc[x]);
-        }
-        __syncthreads();
     }
-    float* o = a.out + row * a.out_stride + h * hd;
-    for (int x = 0; x < 4 && x * 64 + lane < hd; x++) o[x * 64 + lane] = acc[x] / l;
+};
+template <bool Q4, int NB>
+struct VRecord : Record<Q4, NB> {
+    h8 e, w;           // exponents, and 2^-e
+    __device__ __forceinline__ void load(const uint8_t* rec, int lane) {
+        Record<Q4, NB>::load(rec, lane);
+        const uint8_t* tail = rec + NB * (kv_block_bytes(Q4) + 64) + (lane >> 4) * 16;
+        e = *reinterpret_cast<const h8*>(tail);
+        w = *reinterpret_cast<const h8*>(tail + 64);
+    }
+};
+
+// ---- the running softmax of 16 query rows (one per column of the score tiles) ----
+template <int NB>
+struct Tile {
+    h8 qh[NB], ql[NB];
+    float qinv;            // turns an MFMA sum into a score times log2(e)
+    int last, before;      // visible positions: before < p <= last
+    float m, l;            // reference and (the lane's part of the) sum
+    f4 o[2 * NB];          // dims 16 t + 4 g .. + 3 of row `lane & 15`
+
+    // q: the row's head_dim floats (null: an empty row)
+    __device__ __forceinline__ void init(const float* q, int g, float scale) {
+        float x[NB][8], top = 0.f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            f4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
+            if (q) {
+                a = *reinterpret_cast<const f4*>(q + 32 * i + 8 * g);
+                b = *reinterpret_cast<const f4*>(q + 32 * i + 8 * g + 4);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) { x[i][j] = a[j]; x[i][4 + j] = b[j]; }
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[i][j]));
+        }
+        top = fmaxf(top, fx(lane_xor16, top));
+        top = fmaxf(top, fx(lane_xor32, top));
+        int e = 0;
+        if (top > 0.f && top < INFINITY) (void)frexpf(top, &e);
+        e = 13 - e;   // the row's largest lies in [2^12, 2^13)
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i][j] = ldexpf(x[i][j], e);
+            split8(x[i], qh[i], ql[i]);
+        }
+        qinv = ldexpf(scale * 1.44269504088896341f, -e);
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2 * NB; t++) o[t] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // Scores (times log2 e) plus exponents of a record's 32 positions: s[4 t + r] is position 16 t + 4 g + r.
+    template <bool KQ4>
+    __device__ __forceinline__ void scores(const h8 (&kf)[2][NB], const Record<KQ4, NB>& k, const h8& e, float (&s)[8]) const {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            f4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                f4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], ql[i], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], qh[i], c, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) sum[r] = fmaf(c[r], (float)k.d[i][4 * t + r], sum[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * t + r] = fmaf(sum[r], qinv, (float)e[4 * t + r]);
+        }
+    }
+    __device__ __forceinline__ void mask(float (&s)[8], int first, int g) const {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int p = first + (j >> 2) * 16 + g * 4 + (j & 3);
+            if (p > last || p <= before) s[j] = -INFINITY;
+        }
+    }
+    // The probabilities' planes for each block, and the new reference and sum.
+    template <bool VQ4>
+    __device__ __forceinline__ void probabilities(float (&s)[8], const h8& w, h8& ph, h8& pl) {
+        float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        mx = fmaxf(mx, fx(lane_xor16, mx));
+        mx = fmaxf(mx, fx(lane_xor32, mx));
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx);
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < 2 * NB; t++) o[t] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m - P_EXP;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = __builtin_amdgcn_exp2f(s[j] - ref);
+            l = fmaf(p[j], (float)w[j], l);
+        }
+        split8(p, ph, pl);
+    }
+};
+
+struct Part {              // one chunk's result for a row tile, in the workspace
+    float* o;              // [rows][head_dim], unnormalised
+    float* ml;             // [rows][2]: reference and sum
+};
+
+// Work of one launch.  An entry is a tile of query rows with the records it
+// sees; its records are cut into chunks, one workgroup each.
+struct Plan {
+    int rows;              // query rows of a tile
+    int tiles;             // per sequence (own) or of the call (prefix)
+    int entries;           // own: batch * tiles; prefix: tiles
+    int items;             // workgroups per kv head
+    int least;             // records per chunk, at least
+    int whole;             // every entry is one chunk, in the workspace (2) or straight in `out` (1)
+    float *o, *ml;         // workspace: [items][kv_heads][rows] of head_dim and of 2
+};
+
+__device__ __forceinline__ int64_t wave_sum_int(int64_t v) {
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) v += __shfl_xor((long long)v, k);
+    return v;
+}
+
+// Records [x, y) that tile `tile` of sequence b sees of its own slot.
+__device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl, int b, int tile, int group) {
+    const KvSpan sp = kv_span(a.rows, a.cache, b);
+    int i0 = tile * pl.rows / group, i1 = (tile * pl.rows + pl.rows - 1) / group + 1;
+    i0 = i0 < sp.lo ? sp.lo : i0;
+    i1 = i1 > sp.hi ? sp.hi : i1;
+    if (i0 >= i1) return int2{0, 0};
+    const int first = a.window > 0 && sp.start + i0 >= a.window ? sp.start + i0 - a.window + 1 : 0;
+    return int2{first / KV_GROUP, (sp.start + i1 - 1) / KV_GROUP + 1};
+}
+
+// An entry's place among the items: chunks of `size` records, `count` of them from item `first` on.
+struct Cut {
+    int entry, first, count, size;
+};
+// The cut that holds `item`, or (by_entry) the one of entry `item`.  Every
+// wavefront works it out from the lengths in memory: chunks of one size for
+// the whole batch, as small as the items allow, so that long sequences get
+// many workgroups and short ones few.
+__device__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int group, int item, bool by_entry) {
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    for (int e0 = 0; e0 < pl.entries; e0 += 64) {
+        const int e = e0 + lane;
+        int n = 0;
+        if (e < pl.entries) {
+            const int2 r = own_records(a, pl, e / pl.tiles, e % pl.tiles, group);
+            n = r.y - r.x;
+        }
+        total += wave_sum_int(n);
+    }
+    const int spare = pl.items - pl.entries;   // > 0
+    int size = (int)((total + spare - 1) / spare);
+    size = size < pl.least ? pl.least : size;
+    Cut c{-1, 0, 0, size};
+    int before = 0;
+    for (int e0 = 0; e0 < pl.entries; e0 += 64) {
+        const int e = e0 + lane;
+        int n = 0;
+        if (e < pl.entries) {
+            const int2 r = own_records(a, pl, e / pl.tiles, e % pl.tiles, group);
+            n = (r.y - r.x + size - 1) / size;
+        }
+        int upto = n;
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) {
+            const int v = __shfl_up(upto, k);
+            if (lane >= k) upto += v;
+        }
+        const bool mine = by_entry ? e == item : n > 0 && item >= before + upto - n && item < before + upto;
+        const uint64_t who = __ballot(mine);
+        if (who) {
+            const int at = __ffsll((unsigned long long)who) - 1;
+            c.count = __shfl(n, at);
+            c.first = before + __shfl(upto, at) - c.count;
+            c.entry = e0 + at;
+            return c;
+        }
+        before += __shfl(upto, 63);
+    }
+    return c;
+}
+
+// One workgroup: WR x WK wavefronts, each 16 R query rows of a kv head over every
+// WK-th record of the chunk.  Bound by instruction issue where many rows share
+// the records (prompts), by the loads' latency where few do.
+template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE>
+__global__ __launch_bounds__(THREADS) void kv_attention_kernel(KvAttnArgs a, Plan pl) {
+    static_assert(WR * WK == WAVES, "four wavefronts");
+    constexpr int HD = NB * 32, ROWS = 16 * R * WR;
+    const int head = blockIdx.x % a.cache.kv_heads, item = blockIdx.x / a.cache.kv_heads;
+    const int group = a.heads / a.cache.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4;
+    const int wr = wave % WR, wk = wave / WR;
+
+    // which rows and records
+    int b = 0, tile, r0, r1;
+    KvSpan sp{0, 0, 0, 0};
+    if constexpr (PRE) {
+        const int chunks = pl.items / pl.entries, total = (a.prefix_len + KV_GROUP - 1) / KV_GROUP;
+        const int low = a.window > 0 && a.prefix_len >= a.window ? (a.prefix_len - a.window + 1) / KV_GROUP : 0;
+        tile = item / chunks;
+        const int n = total - low, k = item % chunks;
+        r0 = low + (int)((int64_t)n * k / chunks);
+        r1 = low + (int)((int64_t)n * (k + 1) / chunks);
+    } else {
+        if (pl.whole) {
+            // the longest tiles first, and beside each a short one
+            const int half = (pl.tiles + 1) / 2, k = item / a.rows.batch;
+            b = item % a.rows.batch;
+            tile = k < half ? pl.tiles - 1 - k : k - half;
+            const int2 r = own_records(a, pl, b, tile, group);
+            r0 = r.x;
+            r1 = r.y;
+        } else {
+            const Cut c = find_cut(a, pl, group, item, false);
+            if (c.entry < 0) return;
+            b = c.entry / pl.tiles;
+            tile = c.entry % pl.tiles;
+            const int2 r = own_records(a, pl, b, tile, group);
+            r0 = r.x + (item - c.first) * c.size;
+            r1 = r0 + c.size < r.y ? r0 + c.size : r.y;
+        }
+        if (r0 >= r1) return;
+        sp = kv_span(a.rows, a.cache, b);
+    }
+    const KvView& cache = PRE ? a.prefix : a.cache;
+    const int slot = PRE ? a.prefix_slot : sp.slot;
+
+    // the wavefront's query rows
+    Tile<NB> t[R];
+    int64_t out_at[R];     // element of `out` (-1: not a row)
+    int edge_last = 0x7fffffff, edge_before = -1;   // records inside need no mask
+    const int tokens = a.rows.tokens;
+#pragma unroll
+    for (int x = 0; x < R; x++) {
+        const int row = tile * ROWS + (wr * R + x) * 16 + (lane & 15);
+        int i, bb = b;
+        KvSpan s = sp;
+        bool there;
+        if constexpr (PRE) {
+            const int token = row / group;
+            bb = token / tokens;
+            i = token % tokens;
+            there = bb < a.rows.batch;
+            if (there) s = kv_span(a.rows, a.cache, bb);
+        } else {
+            i = row / group;
+            there = i < tokens;
+        }
+        there = there && i >= s.lo && i < s.hi;
+        const int64_t at = (int64_t)bb * tokens + i;
+        const int h = head * group + row % group;
+        out_at[x] = there ? at * a.out_stride + h * HD : -1;
+        t[x].init(there ? a.q + at * a.q_stride + h * HD : nullptr, g, a.scale);
+        // positions in the cache at hand; an empty row sees all of the chunk
+        const int pos = s.start + i;
+        t[x].last = !there ? 0x7fffffff : PRE ? a.prefix_len - 1 : pos;
+        t[x].before = !there || a.window <= 0 ? -1 : (PRE ? a.prefix_len : 0) + pos - a.window;
+        int el = t[x].last, eb = t[x].before;
+#pragma unroll
+        for (int k = 1; k < 16; k *= 2) {
+            const int ol = __shfl_xor(el, k), ob = __shfl_xor(eb, k);
+            el = el < ol ? el : ol;
+            eb = eb > ob ? eb : ob;
+        }
+        el = __builtin_amdgcn_readfirstlane(el);
+        eb = __builtin_amdgcn_readfirstlane(eb);
+        edge_last = el < edge_last ? el : edge_last;
+        edge_before = eb > edge_before ? eb : edge_before;
+    }
+    if (PRE && edge_last > a.prefix_len - 1) edge_last = a.prefix_len - 1;
+
+    const int64_t base = kv_group_index(cache, slot, head, 0);
+    const uint8_t* kb = cache.k + base * cache.k_rec;
+    const uint8_t* vb = cache.v + base * cache.v_rec;
+    constexpr int64_t KREC = kv_record_bytes(KQ4, NB, false), VREC = kv_record_bytes(VQ4, NB, true);
+    Record<KQ4, NB> k;
+    VRecord<VQ4, NB> v;
+    int rec = r0 + wk;
+    if (rec < r1) {
+        k.load(kb + rec * KREC, lane);
+        v.load(vb + rec * VREC, lane);
+    }
+    for (; rec < r1; rec += WK) {
+        const int next = rec + WK < r1 ? rec + WK : rec;
+        float s[R][8];
+        {
+            h8 kf[2][NB];
+#pragma unroll
+            for (int i = 0; i < NB; i++) { kf[0][i] = k.q[i].k(0); kf[1][i] = k.q[i].k(1); }
+#pragma unroll
+            for (int x = 0; x < R; x++) t[x].scores(kf, k, v.e, s[x]);
+        }
+        k.load(kb + next * KREC, lane);
+        if (rec * KV_GROUP + KV_GROUP - 1 > edge_last || rec * KV_GROUP <= edge_before) {
+#pragma unroll
+            for (int x = 0; x < R; x++) t[x].mask(s[x], rec * KV_GROUP, g);
+        }
+        h8 ph[R], pl8[R];
+#pragma unroll
+        for (int x = 0; x < R; x++) t[x].template probabilities<VQ4>(s[x], v.w, ph[x], pl8[x]);
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const h8 d = v.d[i] * v.w;
+            const h8 v0 = v.q[i].v(0), v1 = v.q[i].v(1);
+#pragma unroll
+            for (int x = 0; x < R; x++) {
+                const h8 hi = ph[x] * d;
+                const h8 lo = __builtin_elementwise_fma(pl8[x], d, __builtin_elementwise_fma(ph[x], d, -hi));
+                t[x].o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, hi, t[x].o[2 * i], 0, 0, 0);
+                t[x].o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, hi, t[x].o[2 * i + 1], 0, 0, 0);
+                t[x].o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, lo, t[x].o[2 * i], 0, 0, 0);
+                t[x].o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, lo, t[x].o[2 * i + 1], 0, 0, 0);
+            }
+        }
+        v.load(vb + next * VREC, lane);
+    }
+#pragma unroll
+    for (int x = 0; x < R; x++) {
+        t[x].l += fx(lane_xor16, t[x].l);
+        t[x].l += fx(lane_xor32, t[x].l);
+    }
+
+    if constexpr (WK > 1) {
+        // the wavefronts' records meet in LDS: wavefront 0 of each row set sums them in order
+        constexpr int PITCH = HD + 4;
+        __shared__ float so[WAVES][16 * R][PITCH];
+        __shared__ float sm[WAVES][16 * R][2];
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            const int row = x * 16 + (lane & 15);
+            if (g == 0) { sm[wave][row][0] = t[x].m; sm[wave][row][1] = t[x].l; }
+#pragma unroll
+            for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(&so[wave][row][16 * d + 4 * g]) = t[x].o[d];
+        }
+        __syncthreads();
+        // each wavefront sums a share of the dims
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            const int row = x * 16 + (lane & 15);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WK; w++) mx = fmaxf(mx, sm[wr + w * WR][row][0]);
+            float sum = 0.f, f[WK];
+#pragma unroll
+            for (int w = 0; w < WK; w++) {
+                const float mw = sm[wr + w * WR][row][0];
+                f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx);
+                // a wavefront whose numbers are not numbers passes them on
+                if (mw == -INFINITY && !(sm[wr + w * WR][row][1] == 0.f)) f[w] = 1.f;
+                sum = fmaf(f[w], sm[wr + w * WR][row][1], sum);
+            }
+            const int trow = wr * R * 16 + row;
+            const int64_t part = ((int64_t)item * a.cache.kv_heads + head) * ROWS + trow;
+            const float inv = 1.f / sum;
+            for (int d = wk; d < 2 * NB; d += WK) {
+                f4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < WK; w++)
+                    acc += f[w] * *reinterpret_cast<const f4*>(&so[wr + w * WR][row][16 * d + 4 * g]);
+                if (pl.whole == 1) {
+                    if (out_at[x] >= 0) *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = acc * inv;
+                } else if (out_at[x] >= 0) {
+                    *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = acc;
+                }
+            }
+            if (pl.whole != 1 && out_at[x] >= 0 && wk == 0 && g == 0)
+                *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{mx, sum};
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            if (out_at[x] < 0) continue;
+            if (pl.whole == 1) {
+                const float inv = 1.f / t[x].l;
+#pragma unroll
+                for (int d = 0; d < 2 * NB; d++)
+                    *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = t[x].o[d] * inv;
+            } else {
+                const int trow = (wr * R + x) * 16 + (lane & 15);
+                const int64_t part = ((int64_t)item * a.cache.kv_heads + head) * ROWS + trow;
+#pragma unroll
+                for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = t[x].o[d];
+                if (g == 0) *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{t[x].m, t[x].l};
+            }
+        }
+    }
+}
+
+// The chunks of each row, summed in order: the prefix's, then the row's own.
+// One thread per four dims of a row.
+__global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan own, Plan pre) {
+    const int kvh = a.cache.kv_heads, group = a.heads / kvh, hd = a.cache.head_dim;
+    // one workgroup per entry, kv head and slab of rows
+    const int per = THREADS / (hd / 4) > own.rows ? own.rows : THREADS / (hd / 4);   // rows of a workgroup
+    const int slabs = (own.rows + per - 1) / per;
+    int x = blockIdx.x;
+    const int slab = x % slabs;
+    x /= slabs;
+    const int head = x % kvh, entry = x / kvh;
+    const int b = entry / own.tiles, tile = entry % own.tiles;
+    Cut c{entry, entry, 1, 0};
+    if (!own.whole) c = find_cut(a, own, group, entry, true);
+    else {
+        // whole entries with a prefix: their item is the order that the kernel takes them in
+        const int half = (own.tiles + 1) / 2;
+        const int k = tile >= own.tiles - half ? own.tiles - 1 - tile : tile + half;
+        c.first = k * a.rows.batch + b;
+    }
+    const int trow = slab * per + threadIdx.x / (hd / 4), d = threadIdx.x % (hd / 4) * 4;
+    const int row = tile * own.rows + trow, i = row / group;
+    if (threadIdx.x / (hd / 4) >= per || trow >= own.rows) return;
+    const KvSpan sp = kv_span(a.rows, a.cache, b);
+    if (i < sp.lo || i >= sp.hi) return;
+    const int prow = (b * a.rows.tokens + i) * group + row % group;
+    const int pchunks = pre.items ? pre.items / pre.entries : 0, ptile = pre.items ? prow / pre.rows : 0;
+    const int n = pchunks + c.count;
+    auto part = [&](int k) {
+        return k < pchunks ? ((int64_t)(ptile * pchunks + k) * kvh + head) * pre.rows + prow % pre.rows
+                           : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
+    };
+    auto stats = [&](int k) { return *reinterpret_cast<const f2*>((k < pchunks ? pre.ml : own.ml) + part(k) * 2); };
+    float mx = -INFINITY;
+    for (int k = 0; k < n; k++) mx = fmaxf(mx, stats(k)[0]);
+    float sum = 0.f;
+    f4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < n; k++) {
+        const f2 ml = stats(k);
+        float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mx);
+        if (ml[0] == -INFINITY && !(ml[1] == 0.f)) f = 1.f;   // numbers that are none pass
+        sum = fmaf(f, ml[1], sum);
+        acc += f * *reinterpret_cast<const f4*>((k < pchunks ? pre.o : own.o) + part(k) * hd + d);
+    }
+    const int64_t at = ((int64_t)b * a.rows.tokens + i) * a.out_stride + (head * group + row % group) * hd + d;
+    *reinterpret_cast<f4*>(a.out + at) = acc * (1.f / sum);
+}
+
+// ---- host ----
+struct Config {
+    int r, wr, wk;
+};
+// Query rows per workgroup: as many as there are, while the records are shared by all of them.
+Config config_of(int64_t rows, int blocks) {
+    const int r = blocks == 8 ? 1 : 2;
+    if (rows <= 16) return {1, 1, 4};
+    if (rows <= 16 * r) return {r, 1, 4};
+    if (rows <= 32 * r) return {r, 2, 2};
+    return {r, 4, 1};
+}
+
+constexpr int TARGET = 512;        // workgroups: two per CU
+
+struct Plans {
+    Config own_cfg, pre_cfg;
+    Plan own{}, pre{};
+    size_t bytes = 0;
+};
+
+Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len) {
+    Plans p;
+    const int group = heads / c.kv_heads, blocks = c.head_dim / 32;
+    p.own_cfg = config_of((int64_t)tokens * group, blocks);
+    Plan& o = p.own;
+    o.rows = 16 * p.own_cfg.r * p.own_cfg.wr;
+    o.tiles = (int)(((int64_t)tokens * group + o.rows - 1) / o.rows);
+    o.entries = batch * o.tiles;
+    o.least = p.own_cfg.wk;
+    const int64_t most = (c.groups + o.least - 1) / o.least;   // chunks of an entry
+    const int64_t want = TARGET / c.kv_heads;
+    int64_t items = o.entries;
+    if (o.entries < want && most > 1) items = o.entries + (want < o.entries * most ? want : o.entries * most);
+    o.items = (int)items;
+    o.whole = o.items == o.entries;
+    size_t at = 0;
+    auto take = [&](Plan& x) {
+        const size_t rows = (size_t)x.items * c.kv_heads * x.rows;
+        x.o = reinterpret_cast<float*>(at);
+        at += rows * c.head_dim * 4;
+        x.ml = reinterpret_cast<float*>(at);
+        at += (rows * 8 + 15) & ~(size_t)15;
+    };
+    if (prefix) {
+        p.pre_cfg = config_of((int64_t)batch * tokens * group, blocks);
+        Plan& x = p.pre;
+        x.rows = 16 * p.pre_cfg.r * p.pre_cfg.wr;
+        x.tiles = x.entries = (int)(((int64_t)batch * tokens * group + x.rows - 1) / x.rows);
+        x.least = p.pre_cfg.wk;
+        int64_t chunks = x.entries < want ? want / x.entries : 1;
+        if (prefix_len >= 0) {
+            const int64_t n = ((int64_t)prefix_len + KV_GROUP - 1) / KV_GROUP / x.least;
+            chunks = n < 1 ? 1 : n < chunks ? n : chunks;
+        }
+        x.items = (int)(x.entries * chunks);
+        take(x);
+        o.whole = o.items == o.entries ? 2 : 0;
+    }
+    if (o.whole != 1) take(o);
+    p.bytes = at;
+    return p;
+}
+
+void place(Plan& p, uint8_t* work) {
+    p.o = reinterpret_cast<float*>(work + reinterpret_cast<size_t>(p.o));
+    p.ml = reinterpret_cast<float*>(work + reinterpret_cast<size_t>(p.ml));
+}
+
+template <int NB, bool KQ4, bool VQ4, bool PRE>
+void launch_tile(const Config& f, const KvAttnArgs& a, const Plan& pl, hipStream_t s) {
+    const dim3 grid((uint32_t)pl.items * a.cache.kv_heads);
+    constexpr int R = NB == 8 ? 1 : 2;
+    if (f.wr == 1 && f.r == 1) kv_attention_kernel<NB, KQ4, VQ4, 1, 1, 4, PRE><<<grid, THREADS, 0, s>>>(a, pl);
+    else if (f.wr == 1) kv_attention_kernel<NB, KQ4, VQ4, R, 1, 4, PRE><<<grid, THREADS, 0, s>>>(a, pl);
+    else if (f.wr == 2) kv_attention_kernel<NB, KQ4, VQ4, R, 2, 2, PRE><<<grid, THREADS, 0, s>>>(a, pl);
+    else kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, PRE><<<grid, THREADS, 0, s>>>(a, pl);
+}
+
+template <int NB, bool KQ4, bool VQ4>
+hipError_t launch_types(const KvAttnArgs& a, hipStream_t s) {
+    Plans p = make_plans(a.cache, a.heads, a.rows.batch, a.rows.tokens, a.prefix_len > 0, a.prefix_len);
+    place(p.own, a.work);
+    place(p.pre, a.work);
+    if (p.pre.items) launch_tile<NB, KQ4, VQ4, true>(p.pre_cfg, a, p.pre, s);
+    launch_tile<NB, KQ4, VQ4, false>(p.own_cfg, a, p.own, s);
+    if (p.own.whole != 1) {
+        const int per = THREADS / (a.cache.head_dim / 4) > p.own.rows ? p.own.rows : THREADS / (a.cache.head_dim / 4);
+        const int slabs = (p.own.rows + per - 1) / per;
+        kv_attention_join<<<dim3((uint32_t)p.own.entries * a.cache.kv_heads * slabs), THREADS, 0, s>>>(a, p.own, p.pre);
+    }
+    return hipGetLastError();
+}
+
+template <int NB>
+hipError_t launch_blocks(const KvAttnArgs& a, hipStream_t s) {
+    if (a.cache.k_q4) return a.cache.v_q4 ? launch_types<NB, true, true>(a, s) : launch_types<NB, true, false>(a, s);
+    return a.cache.v_q4 ? launch_types<NB, false, true>(a, s) : launch_types<NB, false, false>(a, s);
 }
 
 }  // namespace
@@ -81,12 +653,18 @@ bool kv_attention_supported(int head_dim) {
     return head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256;
 }
 
-size_t kv_attention_workspace(const KvView&, int, int, int, bool) { return 0; }
+size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix) {
+    return make_plans(c, heads, batch, tokens, prefix, -1).bytes;
+}
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
-    const dim3 grid((uint32_t)a.rows.batch * a.rows.tokens * a.heads);
-    kv_attention_simple<<<grid, 64, 0, s>>>(a);
-    return hipGetLastError();
+    switch (a.cache.head_dim) {
+        case 64: return launch_blocks<2>(a, s);
+        case 96: return launch_blocks<3>(a, s);
+        case 128: return launch_blocks<4>(a, s);
+        case 256: return launch_blocks<8>(a, s);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace llmdot

@@ -143,9 +143,11 @@ __global__ __launch_bounds__(WRITE_THREADS) void kv_write_kernel(KvView c, KvRow
     if (tid >= p0 && tid < p1 && !(taken >> tid & 1)) {
         float m = 0.f;
         for (int i = 0; i < blocks; i++) m = fmaxf(m, vscale[tid][i]);
-        int e = -24;   // a row of zeros: the smallest half's
-        if (m > 0.f) (void)frexpf(m, &e);
-        *reinterpret_cast<_Float16*>(vr + blocks * (kv_block_bytes(VQ4) + 64) + kv_row(tid) * 2) = (_Float16)e;
+        int e = -14;
+        if (m > 0x1p-15f) (void)frexpf(m, &e);
+        _Float16* tail = reinterpret_cast<_Float16*>(vr + blocks * (kv_block_bytes(VQ4) + 64)) + kv_row(tid);
+        tail[0] = (_Float16)e;
+        tail[32] = (_Float16)ldexpf(1.f, -e);
     }
 }
 

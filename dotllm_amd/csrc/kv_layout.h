@@ -3,7 +3,8 @@
 // A kv head of a slot is a run of records of 32 positions, K and V apart:
 //   [head_dim / 32 blocks][64 lanes]  integers, 16 bytes a lane (Q8_0) or 8 (Q4_0)
 //   [head_dim / 32 blocks][32]        fp16 scales, one per position
-//   V only: [32]                      fp16 exponent: 2^e > the position's largest |scale| >= 2^(e-1)
+//   V only: [32] fp16 e and [32] fp16 2^-e, where 2^e is past the position's
+//   largest |scale| and half of it is not (e at least -14)
 // so that one 16-byte load per lane is an operand of v_mfma_f32_16x16x32_f16
 // once its bytes are halves, without LDS or lane exchanges: lane (g, c) = (lane
 // >> 4, lane & 15) of a block holds
@@ -27,7 +28,7 @@ constexpr int KV_GROUP = 32;   // positions per record
 
 __host__ __device__ constexpr int kv_block_bytes(bool q4) { return q4 ? 512 : 1024; }
 __host__ __device__ constexpr int kv_record_bytes(bool q4, int blocks, bool v) {
-    return blocks * (kv_block_bytes(q4) + 64) + (v ? 64 : 0);
+    return blocks * (kv_block_bytes(q4) + 64) + (v ? 128 : 0);
 }
 
 // Order of a position within its record's scales.
