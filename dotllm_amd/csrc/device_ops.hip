@@ -63,7 +63,8 @@ int check_array(const char* name, const void* p) {
     return 0;
 }
 
-constexpr int64_t MAX_GRID = (int64_t)1 << 30;   // workgroups of a launch
+// Workgroups of a launch: a grid has fewer than 2^32 threads, 256 to a workgroup here.
+constexpr int64_t MAX_GRID = ((int64_t)1 << 24) - 1;
 
 // No C++ exception crosses the ABI: a message that could not be built is the only one there is.
 template <typename F>
@@ -258,6 +259,7 @@ int check_verify_shape(int batch, int drafts, int vocab) {
     if (batch < 0 || drafts < 0 || vocab <= 0) return ctx_fail(LLMDOT_E_INVALID, "bad batch, drafts or vocabulary");
     if (batch > 65535 || drafts > 1024 || vocab > (1 << 24))
         return ctx_fail(LLMDOT_E_UNSUPPORTED, "at most 65535 sequences, 1024 drafts and 2^24 tokens in a vocabulary");
+    if ((int64_t)batch * (vocab / 2048 + 1) > MAX_GRID) return ctx_fail(LLMDOT_E_UNSUPPORTED, "too many logits in a call");
     return 0;
 }
 }  // namespace

@@ -34,7 +34,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int THREADS = 256, WAVES = 4;
-constexpr float P_EXP = 14.f;   // probabilities are held times 2^14
+constexpr float P_EXP = 6.f, SLACK = 8.f;   // probabilities are held times 2^6, and at most 2^8 times that
 
 // ---- operands ----
 // Bytes b of w (unsigned, off more than the integer) as halves: 0x6400 + b is 1024 + b.
@@ -187,8 +187,10 @@ struct Tile {
         float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         mx = fmaxf(mx, fx(lane_xor16, mx));
         mx = fmaxf(mx, fx(lane_xor32, mx));
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx);
+        // the reference follows the maximum only where it falls too far behind:
+        // sums are rescaled a few times in a walk, not at most records
+        if (__any(mx > m + SLACK)) {
+            const float mn = mx > m + SLACK ? mx : m;
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= f;
@@ -296,7 +298,7 @@ __device__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int group, int item
 // WK-th record of the chunk.  Bound by instruction issue where many rows share
 // the records (prompts), by the loads' latency where few do.
 template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE>
-__global__ __launch_bounds__(THREADS) void kv_attention_kernel(KvAttnArgs a, Plan pl) {
+__global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(KvAttnArgs a, Plan pl) {
     static_assert(WR * WK == WAVES, "four wavefronts");
     constexpr int HD = NB * 32, ROWS = 16 * R * WR;
     const int head = blockIdx.x % a.cache.kv_heads, item = blockIdx.x / a.cache.kv_heads;
@@ -499,52 +501,65 @@ __global__ __launch_bounds__(THREADS) void kv_attention_kernel(KvAttnArgs a, Pla
     }
 }
 
-// The chunks of each row, summed in order: the prefix's, then the row's own.
-// One thread per four dims of a row.
+// The chunks of a row (the prefix's, then its own) joined: one workgroup per row,
+// hd / 4 lanes to a chunk and as many chunks at a time as fit; the order of the
+// sums depends on their number alone.
 __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan own, Plan pre) {
     const int kvh = a.cache.kv_heads, group = a.heads / kvh, hd = a.cache.head_dim;
-    // one workgroup per entry, kv head and slab of rows
-    const int per = THREADS / (hd / 4) > own.rows ? own.rows : THREADS / (hd / 4);   // rows of a workgroup
-    const int slabs = (own.rows + per - 1) / per;
-    int x = blockIdx.x;
-    const int slab = x % slabs;
-    x /= slabs;
-    const int head = x % kvh, entry = x / kvh;
-    const int b = entry / own.tiles, tile = entry % own.tiles;
-    Cut c{entry, entry, 1, 0};
-    if (!own.whole) c = find_cut(a, own, group, entry, true);
-    else {
-        // whole entries with a prefix: their item is the order that the kernel takes them in
-        const int half = (own.tiles + 1) / 2;
-        const int k = tile >= own.tiles - half ? own.tiles - 1 - tile : tile + half;
-        c.first = k * a.rows.batch + b;
-    }
-    const int trow = slab * per + threadIdx.x / (hd / 4), d = threadIdx.x % (hd / 4) * 4;
-    const int row = tile * own.rows + trow, i = row / group;
-    if (threadIdx.x / (hd / 4) >= per || trow >= own.rows) return;
+    const int h = blockIdx.x % a.heads, token = blockIdx.x / a.heads;
+    const int b = token / a.rows.tokens, i = token % a.rows.tokens, head = h / group, hr = h % group;
     const KvSpan sp = kv_span(a.rows, a.cache, b);
     if (i < sp.lo || i >= sp.hi) return;
-    const int prow = (b * a.rows.tokens + i) * group + row % group;
+    const int row = i * group + hr, tile = row / own.rows, trow = row % own.rows;
+    Cut c{0, 0, 1, 0};
+    if (!own.whole) {
+        c = find_cut(a, own, group, b * own.tiles + tile, true);
+    } else {   // the item that takes the entry
+        const int half = (own.tiles + 1) / 2;
+        c.first = (tile >= own.tiles - half ? own.tiles - 1 - tile : tile + half) * a.rows.batch + b;
+    }
+    const int prow = token * group + hr;
     const int pchunks = pre.items ? pre.items / pre.entries : 0, ptile = pre.items ? prow / pre.rows : 0;
     const int n = pchunks + c.count;
-    auto part = [&](int k) {
-        return k < pchunks ? ((int64_t)(ptile * pchunks + k) * kvh + head) * pre.rows + prow % pre.rows
-                           : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
-    };
-    auto stats = [&](int k) { return *reinterpret_cast<const f2*>((k < pchunks ? pre.ml : own.ml) + part(k) * 2); };
-    float mx = -INFINITY;
-    for (int k = 0; k < n; k++) mx = fmaxf(mx, stats(k)[0]);
-    float sum = 0.f;
+
+    const int lanes = hd / 4, sets = THREADS / lanes;
+    const int set = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
+    float m = -INFINITY, l = 0.f;
     f4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < n; k++) {
-        const f2 ml = stats(k);
-        float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mx);
-        if (ml[0] == -INFINITY && !(ml[1] == 0.f)) f = 1.f;   // numbers that are none pass
-        sum = fmaf(f, ml[1], sum);
-        acc += f * *reinterpret_cast<const f4*>((k < pchunks ? pre.o : own.o) + part(k) * hd + d);
+    if (set < sets) {
+#pragma unroll 4
+        for (int k = set; k < n; k += sets) {
+            const bool of_pre = k < pchunks;
+            const int64_t part = of_pre ? ((int64_t)(ptile * pchunks + k) * kvh + head) * pre.rows + prow % pre.rows
+                                        : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
+            const f2 ml = *reinterpret_cast<const f2*>((of_pre ? pre.ml : own.ml) + part * 2);
+            const f4 o = *reinterpret_cast<const f4*>((of_pre ? pre.o : own.o) + part * hd + d);
+            const float mn = fmaxf(m, ml[0]);
+            const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            const float w = ml[0] == mn ? 1.f : __builtin_amdgcn_exp2f(ml[0] - mn);   // -inf twice: nothing, or no numbers
+            l = fmaf(l, f, w * ml[1]);
+            acc = acc * f + o * w;
+            m = mn;
+        }
     }
-    const int64_t at = ((int64_t)b * a.rows.tokens + i) * a.out_stride + (head * group + row % group) * hd + d;
-    *reinterpret_cast<f4*>(a.out + at) = acc * (1.f / sum);
+    __shared__ float so[THREADS * 4], sml[THREADS / 16][2];
+    if (set < sets) {
+        *reinterpret_cast<f4*>(so + set * hd + d) = acc;
+        if (d == 0) { sml[set][0] = m; sml[set][1] = l; }
+    }
+    __syncthreads();
+    if (set != 0) return;
+    const int used = n < sets ? n : sets;
+    for (int k = 1; k < used; k++) {
+        const float mk = sml[k][0], mn = fmaxf(m, mk);
+        const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float w = mk == mn ? 1.f : __builtin_amdgcn_exp2f(mk - mn);
+        l = fmaf(l, f, w * sml[k][1]);
+        acc = acc * f + *reinterpret_cast<const f4*>(so + k * hd + d) * w;
+        m = mn;
+    }
+    const int64_t at = (int64_t)token * a.out_stride + h * hd + d;
+    *reinterpret_cast<f4*>(a.out + at) = acc * (1.f / l);
 }
 
 // ---- host ----
@@ -634,9 +649,8 @@ hipError_t launch_types(const KvAttnArgs& a, hipStream_t s) {
     if (p.pre.items) launch_tile<NB, KQ4, VQ4, true>(p.pre_cfg, a, p.pre, s);
     launch_tile<NB, KQ4, VQ4, false>(p.own_cfg, a, p.own, s);
     if (p.own.whole != 1) {
-        const int per = THREADS / (a.cache.head_dim / 4) > p.own.rows ? p.own.rows : THREADS / (a.cache.head_dim / 4);
-        const int slabs = (p.own.rows + per - 1) / per;
-        kv_attention_join<<<dim3((uint32_t)p.own.entries * a.cache.kv_heads * slabs), THREADS, 0, s>>>(a, p.own, p.pre);
+        const int64_t rows = (int64_t)a.rows.batch * a.rows.tokens * a.heads;
+        kv_attention_join<<<dim3((uint32_t)rows), THREADS, 0, s>>>(a, p.own, p.pre);
     }
     return hipGetLastError();
 }
