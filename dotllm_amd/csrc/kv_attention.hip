@@ -20,6 +20,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace llmdot {
@@ -182,7 +183,6 @@ struct Tile {
         }
     }
     // The probabilities' planes for each block, and the new reference and sum.
-    template <bool VQ4>
     __device__ __forceinline__ void probabilities(float (&s)[8], const h8& w, h8& ph, h8& pl) {
         float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         mx = fmaxf(mx, fx(lane_xor16, mx));
@@ -208,11 +208,6 @@ struct Tile {
     }
 };
 
-struct Part {              // one chunk's result for a row tile, in the workspace
-    float* o;              // [rows][head_dim], unnormalised
-    float* ml;             // [rows][2]: reference and sum
-};
-
 // Work of one launch.  An entry is a tile of query rows with the records it
 // sees; its records are cut into chunks, one workgroup each.
 struct Plan {
@@ -223,13 +218,8 @@ struct Plan {
     int least;             // records per chunk, at least
     int whole;             // every entry is one chunk, in the workspace (2) or straight in `out` (1)
     float *o, *ml;         // workspace: [items][kv_heads][rows] of head_dim and of 2
+    uint32_t* arrived;     // finished chunks of each (entry, kv head), zero between calls
 };
-
-__device__ __forceinline__ int64_t wave_sum_int(int64_t v) {
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) v += __shfl_xor((long long)v, k);
-    return v;
-}
 
 // Records [x, y) that tile `tile` of sequence b sees of its own slot.
 __device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl, int b, int tile, int group) {
@@ -242,80 +232,108 @@ __device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl,
     return int2{first / KV_GROUP, (sp.start + i1 - 1) / KV_GROUP + 1};
 }
 
-// An entry's place among the items: chunks of `size` records, `count` of them from item `first` on.
+// An entry's place among the items: its records [r0, r1) in `count` chunks of
+// `size` from item `first` on.
 struct Cut {
-    int entry, first, count, size;
+    int entry, first, count, size, r0, r1;
 };
-// The cut that holds `item`, or (by_entry) the one of entry `item`.  Every
-// wavefront works it out from the lengths in memory: chunks of one size for
-// the whole batch, as small as the items allow, so that long sequences get
-// many workgroups and short ones few.
-__device__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int group, int item, bool by_entry) {
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+    v += lane_xor1(v);
+    v += lane_xor2(v);
+    v += lane_mirror8(v);
+    v += lane_mirror16(v);
+    v += lane_xor16(v);
+    return v + lane_xor32(v);
+}
+// The cut that holds `item`, or (by_entry) the one of entry `item`; entry -1: an
+// item that no entry needs.  Every wavefront works it out from the lengths in
+// memory: chunks of one size for the whole batch, as small as the items allow,
+// so that long sequences get many workgroups and short ones few.
+__device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int group, int item, bool by_entry) {
+    const uint32_t spare = pl.items - pl.entries;   // > 0
+    if (pl.entries == 1) {
+        const int2 r = own_records(a, pl, 0, 0, group);
+        const int n = r.y - r.x;
+        int size = (int)((n + spare - 1) / spare);
+        size = size < pl.least ? pl.least : size;
+        const int count = (n + size - 1) / size;
+        return Cut{by_entry || item < count ? 0 : -1, 0, count, size, r.x, r.y};
+    }
     const int lane = threadIdx.x & 63;
-    int64_t total = 0;
+    int2 r{0, 0};
+    uint64_t total = 0;
     for (int e0 = 0; e0 < pl.entries; e0 += 64) {
         const int e = e0 + lane;
-        int n = 0;
-        if (e < pl.entries) {
-            const int2 r = own_records(a, pl, e / pl.tiles, e % pl.tiles, group);
-            n = r.y - r.x;
-        }
-        total += wave_sum_int(n);
+        r = e < pl.entries ? own_records(a, pl, e / pl.tiles, e % pl.tiles, group) : int2{0, 0};
+        total += wave_sum_u32((uint32_t)(r.y - r.x));   // at most 64 * 2^25
     }
-    const int spare = pl.items - pl.entries;   // > 0
-    int size = (int)((total + spare - 1) / spare);
+    int size = total >> 32 ? (int)((total + spare - 1) / spare) : (int)(((uint32_t)total + (spare - 1)) / spare);
     size = size < pl.least ? pl.least : size;
-    Cut c{-1, 0, 0, size};
     int before = 0;
     for (int e0 = 0; e0 < pl.entries; e0 += 64) {
         const int e = e0 + lane;
-        int n = 0;
-        if (e < pl.entries) {
-            const int2 r = own_records(a, pl, e / pl.tiles, e % pl.tiles, group);
-            n = (r.y - r.x + size - 1) / size;
-        }
+        if (pl.entries > 64) r = e < pl.entries ? own_records(a, pl, e / pl.tiles, e % pl.tiles, group) : int2{0, 0};
+        const int n = (r.y - r.x + size - 1) / size;
         int upto = n;
 #pragma unroll
         for (int k = 1; k < 64; k *= 2) {
             const int v = __shfl_up(upto, k);
             if (lane >= k) upto += v;
         }
-        const bool mine = by_entry ? e == item : n > 0 && item >= before + upto - n && item < before + upto;
+        const bool mine = by_entry ? e == item : item >= before + upto - n && item < before + upto;
         const uint64_t who = __ballot(mine);
         if (who) {
-            const int at = __ffsll((unsigned long long)who) - 1;
-            c.count = __shfl(n, at);
-            c.first = before + __shfl(upto, at) - c.count;
-            c.entry = e0 + at;
-            return c;
+            const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
+            const int count = __builtin_amdgcn_readlane(n, at);
+            return Cut{e0 + at, before + __builtin_amdgcn_readlane(upto, at) - count, count, size,
+                       __builtin_amdgcn_readlane(r.x, at), __builtin_amdgcn_readlane(r.y, at)};
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return c;
+    return Cut{-1, 0, 0, size, 0, 0};
+}
+
+// Partial results cross XCDs inside a launch (the last workgroup of an entry
+// joins it): written through, and read past, the XCD's own L2.
+__device__ __forceinline__ void store_through(float* p, f2 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f2 load_past(const float* p) {
+    return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// (reference, sum) pairs and what they weigh joined: running values times f, the new ones times w.
+__device__ __forceinline__ void join_weights(float& m, float mk, float& f, float& w) {
+    const float mn = fmaxf(m, mk);
+    f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+    w = mk == mn ? 1.f : __builtin_amdgcn_exp2f(mk - mn);   // -inf twice: nothing, or what is no number
+    m = mn;
 }
 
 // One workgroup: WR x WK wavefronts, each 16 R query rows of a kv head over every
 // WK-th record of the chunk.  Bound by instruction issue where many rows share
-// the records (prompts), by the loads' latency where few do.
-template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE>
-__global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(KvAttnArgs a, Plan pl) {
+// the records (prompts), by the loads' latency where few do.  FUSE: the
+// workgroup that finishes an entry's last chunk joins them.
+template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE, bool FUSE>
+__device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl, int wg, float* lds) {
     static_assert(WR * WK == WAVES, "four wavefronts");
     constexpr int HD = NB * 32, ROWS = 16 * R * WR;
-    const int head = blockIdx.x % a.cache.kv_heads, item = blockIdx.x / a.cache.kv_heads;
-    const int group = a.heads / a.cache.kv_heads;
+    const int kvh = a.cache.kv_heads, head = wg % kvh, item = wg / kvh, group = a.heads / kvh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4;
     const int wr = wave % WR, wk = wave / WR;
 
     // which rows and records
-    int b = 0, tile, r0, r1;
+    int b = 0, tile, r0, r1, entry = 0, chunks = 1, first_item = item;
     KvSpan sp{0, 0, 0, 0};
     if constexpr (PRE) {
-        const int chunks = pl.items / pl.entries, total = (a.prefix_len + KV_GROUP - 1) / KV_GROUP;
+        const int per = pl.items / pl.entries, total = (a.prefix_len + KV_GROUP - 1) / KV_GROUP;
         const int low = a.window > 0 && a.prefix_len >= a.window ? (a.prefix_len - a.window + 1) / KV_GROUP : 0;
-        tile = item / chunks;
-        const int n = total - low, k = item % chunks;
-        r0 = low + (int)((int64_t)n * k / chunks);
-        r1 = low + (int)((int64_t)n * (k + 1) / chunks);
+        tile = item / per;
+        const int n = total - low, k = item % per;
+        r0 = low + (int)((int64_t)n * k / per);
+        r1 = low + (int)((int64_t)n * (k + 1) / per);
     } else {
         if (pl.whole) {
             // the longest tiles first, and beside each a short one
@@ -328,17 +346,30 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
         } else {
             const Cut c = find_cut(a, pl, group, item, false);
             if (c.entry < 0) return;
-            b = c.entry / pl.tiles;
-            tile = c.entry % pl.tiles;
-            const int2 r = own_records(a, pl, b, tile, group);
-            r0 = r.x + (item - c.first) * c.size;
-            r1 = r0 + c.size < r.y ? r0 + c.size : r.y;
+            entry = c.entry;
+            chunks = c.count;
+            first_item = c.first;
+            b = entry / pl.tiles;
+            tile = entry % pl.tiles;
+            r0 = c.r0 + (item - c.first) * c.size;
+            r1 = r0 + c.size < c.r1 ? r0 + c.size : c.r1;
         }
         if (r0 >= r1) return;
         sp = kv_span(a.rows, a.cache, b);
     }
     const KvView& cache = PRE ? a.prefix : a.cache;
     const int slot = PRE ? a.prefix_slot : sp.slot;
+    const int64_t base = kv_group_index(cache, slot, head, 0);
+    const uint8_t* kb = cache.k + base * cache.k_rec;
+    const uint8_t* vb = cache.v + base * cache.v_rec;
+    constexpr int64_t KREC = kv_record_bytes(KQ4, NB, false), VREC = kv_record_bytes(VQ4, NB, true);
+    Record<KQ4, NB> k;
+    VRecord<VQ4, NB> v;
+    int rec = r0 + wk;
+    if (rec < r1) {
+        k.load(kb + rec * KREC, lane);
+        v.load(vb + rec * VREC, lane);
+    }
 
     // the wavefront's query rows
     Tile<NB> t[R];
@@ -384,17 +415,6 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
     }
     if (PRE && edge_last > a.prefix_len - 1) edge_last = a.prefix_len - 1;
 
-    const int64_t base = kv_group_index(cache, slot, head, 0);
-    const uint8_t* kb = cache.k + base * cache.k_rec;
-    const uint8_t* vb = cache.v + base * cache.v_rec;
-    constexpr int64_t KREC = kv_record_bytes(KQ4, NB, false), VREC = kv_record_bytes(VQ4, NB, true);
-    Record<KQ4, NB> k;
-    VRecord<VQ4, NB> v;
-    int rec = r0 + wk;
-    if (rec < r1) {
-        k.load(kb + rec * KREC, lane);
-        v.load(vb + rec * VREC, lane);
-    }
     for (; rec < r1; rec += WK) {
         const int next = rec + WK < r1 ? rec + WK : rec;
         float s[R][8];
@@ -412,7 +432,7 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
         }
         h8 ph[R], pl8[R];
 #pragma unroll
-        for (int x = 0; x < R; x++) t[x].template probabilities<VQ4>(s[x], v.w, ph[x], pl8[x]);
+        for (int x = 0; x < R; x++) t[x].probabilities(s[x], v.w, ph[x], pl8[x]);
 #pragma unroll
         for (int i = 0; i < NB; i++) {
             const h8 d = v.d[i] * v.w;
@@ -435,11 +455,11 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
         t[x].l += fx(lane_xor32, t[x].l);
     }
 
+    const bool direct = pl.whole == 1 || (FUSE && chunks == 1);
     if constexpr (WK > 1) {
-        // the wavefronts' records meet in LDS: wavefront 0 of each row set sums them in order
-        constexpr int PITCH = HD + 4;
-        __shared__ float so[WAVES][16 * R][PITCH];
-        __shared__ float sm[WAVES][16 * R][2];
+        // the wavefronts' records meet in LDS, each wavefront summing a share of the dims in order
+        auto so = reinterpret_cast<float (*)[16 * R][HD + 4]>(lds);
+        auto sm = reinterpret_cast<float (*)[16 * R][2]>(lds + WAVES * 16 * R * (HD + 4));
 #pragma unroll
         for (int x = 0; x < R; x++) {
             const int row = x * 16 + (lane & 15);
@@ -448,56 +468,131 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
             for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(&so[wave][row][16 * d + 4 * g]) = t[x].o[d];
         }
         __syncthreads();
-        // each wavefront sums a share of the dims
 #pragma unroll
         for (int x = 0; x < R; x++) {
             const int row = x * 16 + (lane & 15);
-            float mx = -INFINITY;
+            float mx = -INFINITY, sum = 0.f, f[WK];
 #pragma unroll
             for (int w = 0; w < WK; w++) mx = fmaxf(mx, sm[wr + w * WR][row][0]);
-            float sum = 0.f, f[WK];
 #pragma unroll
             for (int w = 0; w < WK; w++) {
                 const float mw = sm[wr + w * WR][row][0];
-                f[w] = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mx);
-                // a wavefront whose numbers are not numbers passes them on
-                if (mw == -INFINITY && !(sm[wr + w * WR][row][1] == 0.f)) f[w] = 1.f;
+                f[w] = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
                 sum = fmaf(f[w], sm[wr + w * WR][row][1], sum);
             }
-            const int trow = wr * R * 16 + row;
-            const int64_t part = ((int64_t)item * a.cache.kv_heads + head) * ROWS + trow;
+            const int64_t part = ((int64_t)item * kvh + head) * ROWS + wr * R * 16 + row;
             const float inv = 1.f / sum;
+            if (out_at[x] < 0) continue;
             for (int d = wk; d < 2 * NB; d += WK) {
                 f4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < WK; w++)
                     acc += f[w] * *reinterpret_cast<const f4*>(&so[wr + w * WR][row][16 * d + 4 * g]);
-                if (pl.whole == 1) {
-                    if (out_at[x] >= 0) *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = acc * inv;
-                } else if (out_at[x] >= 0) {
-                    *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = acc;
+                float* o = pl.o + part * HD + 16 * d + 4 * g;
+                if (direct) {
+                    *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = acc * inv;
+                } else if constexpr (FUSE) {
+                    store_through(o, f2{acc[0], acc[1]});
+                    store_through(o + 2, f2{acc[2], acc[3]});
+                } else {
+                    *reinterpret_cast<f4*>(o) = acc;
                 }
             }
-            if (pl.whole != 1 && out_at[x] >= 0 && wk == 0 && g == 0)
-                *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{mx, sum};
+            if (!direct && wk == 0 && g == 0) {
+                if constexpr (FUSE) store_through(pl.ml + part * 2, f2{mx, sum});
+                else *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{mx, sum};
+            }
         }
     } else {
 #pragma unroll
         for (int x = 0; x < R; x++) {
             if (out_at[x] < 0) continue;
-            if (pl.whole == 1) {
+            if (direct) {
                 const float inv = 1.f / t[x].l;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; d++)
                     *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = t[x].o[d] * inv;
             } else {
                 const int trow = (wr * R + x) * 16 + (lane & 15);
-                const int64_t part = ((int64_t)item * a.cache.kv_heads + head) * ROWS + trow;
+                const int64_t part = ((int64_t)item * kvh + head) * ROWS + trow;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = t[x].o[d];
                 if (g == 0) *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{t[x].m, t[x].l};
             }
         }
+    }
+
+    if constexpr (FUSE) {
+        if (direct) return;
+        // every store of this workgroup is past the L2 before it counts itself in
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        int& is_last = *reinterpret_cast<int*>(lds + WAVES * 16 * R * (HD + 6));
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            uint32_t* count = pl.arrived + entry * kvh + head;
+            const uint32_t was = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            is_last = was + 1 == (uint32_t)chunks;
+            if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!is_last) return;
+        // rows x (HD / 4) lanes, the chunks of a row in as many sets as the threads allow
+        constexpr int LANES = HD / 4, SETS = THREADS / LANES;
+        const int set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+        const int i0 = tile * ROWS / group, i1 = (tile * ROWS + ROWS - 1) / group + 1;
+        const int lo = (sp.lo > i0 ? sp.lo : i0) * group, hi = (sp.hi < i1 ? sp.hi : i1) * group;   // its rows
+        const int begin = lo > tile * ROWS ? lo - tile * ROWS : 0, end = hi - tile * ROWS < ROWS ? hi - tile * ROWS : ROWS;
+        const int rows = end - begin;
+        const int share = SETS / rows > 1 ? SETS / rows : 1;       // sets that split a row's chunks
+        auto jo = reinterpret_cast<float (*)[HD]>(lds);
+        auto jm = reinterpret_cast<float (*)[2]>(lds + SETS * HD);
+        for (int q0 = 0; q0 < rows; q0 += SETS / share) {
+            const int q = q0 + set / share, part_of = set % share;
+            const bool on = set < SETS / share * share && q < rows;
+            float m = -INFINITY, l = 0.f;
+            f4 acc{0.f, 0.f, 0.f, 0.f};
+            if (on) {
+#pragma unroll 4
+                for (int c = part_of; c < chunks; c += share) {
+                    const int64_t part = ((int64_t)(first_item + c) * kvh + head) * ROWS + begin + q;
+                    const f2 ml = load_past(pl.ml + part * 2);
+                    const f2 oa = load_past(pl.o + part * HD + d), ob = load_past(pl.o + part * HD + d + 2);
+                    float f, w;
+                    join_weights(m, ml[0], f, w);
+                    l = fmaf(l, f, w * ml[1]);
+                    acc = acc * f + f4{oa[0], oa[1], ob[0], ob[1]} * w;
+                }
+                *reinterpret_cast<f4*>(&jo[set][d]) = acc;
+                if (d == 0) { jm[set][0] = m; jm[set][1] = l; }
+            }
+            __syncthreads();
+            if (on && part_of == 0) {
+                for (int c = 1; c < share && c < chunks; c++) {
+                    float f, w;
+                    join_weights(m, jm[set + c][0], f, w);
+                    l = fmaf(l, f, w * jm[set + c][1]);
+                    acc = acc * f + *reinterpret_cast<const f4*>(&jo[set + c][d]) * w;
+                }
+                const int row = tile * ROWS + begin + q;
+                const int64_t at = ((int64_t)b * tokens + row / group) * a.out_stride + (head * group + row % group) * HD;
+                *reinterpret_cast<f4*>(a.out + at + d) = acc * (1.f / l);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// The call's own chunks, and (RP) the prefix's before them, 16 RP rows to a wavefront.
+template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, int RP>
+__global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(KvAttnArgs a, Plan own, Plan pre) {
+    constexpr int MOST = RP > (WK > 1 ? R : 0) ? RP : WK > 1 ? R : 0;   // tiles of a wavefront that meet in LDS
+    __shared__ __align__(16) float lds[MOST > 0 ? WAVES * 16 * MOST * (NB * 32 + 6) + 4 : 4];
+    if constexpr (RP > 0) {
+        const int before = pre.items * a.cache.kv_heads;
+        if ((int)blockIdx.x < before) attend_chunk<NB, KQ4, VQ4, RP, 1, 4, true, false>(a, pre, blockIdx.x, lds);
+        else attend_chunk<NB, KQ4, VQ4, R, WR, WK, false, false>(a, own, blockIdx.x - before, lds);
+    } else {
+        attend_chunk<NB, KQ4, VQ4, R, WR, WK, false, R == 1 && WK == 4>(a, own, blockIdx.x, lds);
     }
 }
 
@@ -511,7 +606,7 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     const KvSpan sp = kv_span(a.rows, a.cache, b);
     if (i < sp.lo || i >= sp.hi) return;
     const int row = i * group + hr, tile = row / own.rows, trow = row % own.rows;
-    Cut c{0, 0, 1, 0};
+    Cut c{0, 0, 1, 0, 0, 0};
     if (!own.whole) {
         c = find_cut(a, own, group, b * own.tiles + tile, true);
     } else {   // the item that takes the entry
@@ -534,12 +629,10 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
                                         : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
             const f2 ml = *reinterpret_cast<const f2*>((of_pre ? pre.ml : own.ml) + part * 2);
             const f4 o = *reinterpret_cast<const f4*>((of_pre ? pre.o : own.o) + part * hd + d);
-            const float mn = fmaxf(m, ml[0]);
-            const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            const float w = ml[0] == mn ? 1.f : __builtin_amdgcn_exp2f(ml[0] - mn);   // -inf twice: nothing, or no numbers
+            float f, w;
+            join_weights(m, ml[0], f, w);
             l = fmaf(l, f, w * ml[1]);
             acc = acc * f + o * w;
-            m = mn;
         }
     }
     __shared__ float so[THREADS * 4], sml[THREADS / 16][2];
@@ -551,12 +644,10 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     if (set != 0) return;
     const int used = n < sets ? n : sets;
     for (int k = 1; k < used; k++) {
-        const float mk = sml[k][0], mn = fmaxf(m, mk);
-        const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        const float w = mk == mn ? 1.f : __builtin_amdgcn_exp2f(mk - mn);
+        float f, w;
+        join_weights(m, sml[k][0], f, w);
         l = fmaf(l, f, w * sml[k][1]);
         acc = acc * f + *reinterpret_cast<const f4*>(so + k * hd + d) * w;
-        m = mn;
     }
     const int64_t at = (int64_t)token * a.out_stride + h * hd + d;
     *reinterpret_cast<f4*>(a.out + at) = acc * (1.f / l);
@@ -566,89 +657,87 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
 struct Config {
     int r, wr, wk;
 };
-// Query rows per workgroup: as many as there are, while the records are shared by all of them.
-Config config_of(int64_t rows, int blocks) {
-    const int r = blocks == 8 ? 1 : 2;
-    if (rows <= 16) return {1, 1, 4};
-    if (rows <= 16 * r) return {r, 1, 4};
-    if (rows <= 32 * r) return {r, 2, 2};
-    return {r, 4, 1};
-}
-
+constexpr int PRE_R = 2;
 constexpr int TARGET = 512;        // workgroups: two per CU
+constexpr size_t ARRIVED_BYTES = 4 * 2 * TARGET;   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
-    Config own_cfg, pre_cfg;
+    Config own_cfg;
     Plan own{}, pre{};
+    bool fused;
     size_t bytes = 0;
 };
 
-Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len) {
+int rows_per_wave(int blocks) { return blocks == 8 ? 1 : 2; }   // tiles of 16: registers for two wavefronts per SIMD
+
+// Shapes of the launch, from sizes that the host knows (lengths are on the
+// device).  16 rows or fewer (decode): four wavefronts share the keys of one
+// tile.  More: four wavefronts of 32 rows each over the same keys where that
+// gives a workgroup for every CU, else one such tile per workgroup, its keys
+// over the wavefronts and, in chunks, over workgroups.
+Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len, uint8_t* work) {
     Plans p;
-    const int group = heads / c.kv_heads, blocks = c.head_dim / 32;
-    p.own_cfg = config_of((int64_t)tokens * group, blocks);
+    const int group = heads / c.kv_heads, r = rows_per_wave(c.head_dim / 32);
+    const int64_t rows = (int64_t)tokens * group, want = TARGET / c.kv_heads;
+    auto tiles_of = [](int64_t n, int per) { return (int)((n + per - 1) / per); };
+    if (rows <= 16) p.own_cfg = {1, 1, 4};
+    else if ((int64_t)batch * tiles_of(rows, 64 * r) * c.kv_heads >= TARGET / 2) p.own_cfg = {r, 4, 1};
+    else p.own_cfg = {r, 1, 4};
     Plan& o = p.own;
     o.rows = 16 * p.own_cfg.r * p.own_cfg.wr;
-    o.tiles = (int)(((int64_t)tokens * group + o.rows - 1) / o.rows);
+    o.tiles = tiles_of(rows, o.rows);
     o.entries = batch * o.tiles;
     o.least = p.own_cfg.wk;
-    const int64_t most = (c.groups + o.least - 1) / o.least;   // chunks of an entry
-    const int64_t want = TARGET / c.kv_heads;
-    int64_t items = o.entries;
-    if (o.entries < want && most > 1) items = o.entries + (want < o.entries * most ? want : o.entries * most);
-    o.items = (int)items;
-    o.whole = o.items == o.entries;
+    const int64_t most = tiles_of(c.groups, o.least);   // chunks of an entry
+    o.items = o.entries;
+    if (p.own_cfg.wk > 1 && o.entries < want && most > 1) o.items += (int)std::min(want, o.entries * most);
+    o.whole = o.items == o.entries ? prefix ? 2 : 1 : 0;
+    p.fused = !prefix && p.own_cfg.r == 1 && p.own_cfg.wk == 4 && !o.whole;
     size_t at = 0;
-    auto take = [&](Plan& x) {
-        const size_t rows = (size_t)x.items * c.kv_heads * x.rows;
-        x.o = reinterpret_cast<float*>(at);
-        at += rows * c.head_dim * 4;
-        x.ml = reinterpret_cast<float*>(at);
-        at += (rows * 8 + 15) & ~(size_t)15;
+    auto take = [&](size_t n) {
+        uint8_t* q = work + at;
+        at += (n + 15) & ~(size_t)15;
+        return q;
     };
+    auto take_parts = [&](Plan& x) {
+        const size_t n = (size_t)x.items * c.kv_heads * x.rows;
+        x.o = reinterpret_cast<float*>(take(n * c.head_dim * 4));
+        x.ml = reinterpret_cast<float*>(take(n * 8));
+    };
+    // the counters come first in every workspace: what a call leaves there is zero for any other
+    o.arrived = reinterpret_cast<uint32_t*>(take(ARRIVED_BYTES));
     if (prefix) {
-        p.pre_cfg = config_of((int64_t)batch * tokens * group, blocks);
         Plan& x = p.pre;
-        x.rows = 16 * p.pre_cfg.r * p.pre_cfg.wr;
-        x.tiles = x.entries = (int)(((int64_t)batch * tokens * group + x.rows - 1) / x.rows);
-        x.least = p.pre_cfg.wk;
+        x.rows = 16 * std::min(PRE_R, r);
+        x.tiles = x.entries = tiles_of(batch * rows, x.rows);
+        x.least = 4;
         int64_t chunks = x.entries < want ? want / x.entries : 1;
-        if (prefix_len >= 0) {
-            const int64_t n = ((int64_t)prefix_len + KV_GROUP - 1) / KV_GROUP / x.least;
-            chunks = n < 1 ? 1 : n < chunks ? n : chunks;
-        }
+        if (prefix_len >= 0) chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, tiles_of(prefix_len, KV_GROUP) / x.least));
         x.items = (int)(x.entries * chunks);
-        take(x);
-        o.whole = o.items == o.entries ? 2 : 0;
+        take_parts(x);
     }
-    if (o.whole != 1) take(o);
+    if (o.whole != 1) take_parts(o);
     p.bytes = at;
     return p;
 }
 
-void place(Plan& p, uint8_t* work) {
-    p.o = reinterpret_cast<float*>(work + reinterpret_cast<size_t>(p.o));
-    p.ml = reinterpret_cast<float*>(work + reinterpret_cast<size_t>(p.ml));
-}
-
-template <int NB, bool KQ4, bool VQ4, bool PRE>
-void launch_tile(const Config& f, const KvAttnArgs& a, const Plan& pl, hipStream_t s) {
-    const dim3 grid((uint32_t)pl.items * a.cache.kv_heads);
+template <int NB, bool KQ4, bool VQ4, int RP>
+void launch_own(const Plans& p, const KvAttnArgs& a, hipStream_t s) {
+    const dim3 grid((uint32_t)((p.own.items + p.pre.items) * a.cache.kv_heads));
     constexpr int R = NB == 8 ? 1 : 2;
-    if (f.wr == 1 && f.r == 1) kv_attention_kernel<NB, KQ4, VQ4, 1, 1, 4, PRE><<<grid, THREADS, 0, s>>>(a, pl);
-    else if (f.wr == 1) kv_attention_kernel<NB, KQ4, VQ4, R, 1, 4, PRE><<<grid, THREADS, 0, s>>>(a, pl);
-    else if (f.wr == 2) kv_attention_kernel<NB, KQ4, VQ4, R, 2, 2, PRE><<<grid, THREADS, 0, s>>>(a, pl);
-    else kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, PRE><<<grid, THREADS, 0, s>>>(a, pl);
+    const Config& f = p.own_cfg;
+    if (a.rows.tokens * (a.heads / a.cache.kv_heads) <= 16)
+        kv_attention_kernel<NB, KQ4, VQ4, 1, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
+    else if (f.wr == 1) kv_attention_kernel<NB, KQ4, VQ4, R, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
+    else kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
 }
 
 template <int NB, bool KQ4, bool VQ4>
 hipError_t launch_types(const KvAttnArgs& a, hipStream_t s) {
-    Plans p = make_plans(a.cache, a.heads, a.rows.batch, a.rows.tokens, a.prefix_len > 0, a.prefix_len);
-    place(p.own, a.work);
-    place(p.pre, a.work);
-    if (p.pre.items) launch_tile<NB, KQ4, VQ4, true>(p.pre_cfg, a, p.pre, s);
-    launch_tile<NB, KQ4, VQ4, false>(p.own_cfg, a, p.own, s);
-    if (p.own.whole != 1) {
+    const Plans p = make_plans(a.cache, a.heads, a.rows.batch, a.rows.tokens, a.prefix_len > 0, a.prefix_len, a.work);
+    if (p.pre.items) launch_own<NB, KQ4, VQ4, NB == 8 ? 1 : PRE_R>(p, a, s);
+    else launch_own<NB, KQ4, VQ4, 0>(p, a, s);
+    if (p.own.whole != 1 && !p.fused) {
         const int64_t rows = (int64_t)a.rows.batch * a.rows.tokens * a.heads;
         kv_attention_join<<<dim3((uint32_t)rows), THREADS, 0, s>>>(a, p.own, p.pre);
     }
@@ -668,7 +757,7 @@ bool kv_attention_supported(int head_dim) {
 }
 
 size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix) {
-    return make_plans(c, heads, batch, tokens, prefix, -1).bytes;
+    return make_plans(c, heads, batch, tokens, prefix, -1, nullptr).bytes;
 }
 
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {

@@ -16,7 +16,8 @@
  *     kernels: nothing outside the cache or the arrays is read or written.
  *   - A workspace belongs to one call until that call's kernels have run: calls
  *     in the order of one stream may share it, graphs replayed at the same time
- *     may not.  Its contents on entry do not matter.
+ *     may not.  It is zeroed once before its first call (llmdot_hip_device_alloc
+ *     does that); every call leaves it fit for the next, whatever its sizes.
  *   - No counterpart in the reference, whose cache is fp32 and whose loop holds
  *     one sequence (src/Llmdot.Core/Inference/KvCache.cs).
  */
