@@ -317,6 +317,7 @@ struct KvAttnArgs {
     int prefix_slot, prefix_len;
     float scale;
     uint8_t* work;            // kv_attention_workspace bytes
+    Divisor by_group, by_tokens, by_kv_heads;   // set by the launcher
 };
 bool kv_attention_supported(int head_dim);
 size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix);

@@ -215,16 +215,17 @@ struct Plan {
     int tiles;             // per sequence (own) or of the call (prefix)
     int entries;           // own: batch * tiles; prefix: tiles
     int items;             // workgroups per kv head
-    int least;             // records per chunk, at least
+    int least;             // records per chunk, at least, as a rule
+    Divisor by_tiles, by_batch;
+    float per_record;      // chunks per record, at most
     int whole;             // every entry is one chunk, in the workspace (2) or straight in `out` (1)
     float *o, *ml;         // workspace: [items][kv_heads][rows] of head_dim and of 2
     uint32_t* arrived;     // finished chunks of each (entry, kv head), zero between calls
 };
 
 // Records [x, y) that tile `tile` of sequence b sees of its own slot.
-__device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl, int b, int tile, int group) {
-    const KvSpan sp = kv_span(a.rows, a.cache, b);
-    int i0 = tile * pl.rows / group, i1 = (tile * pl.rows + pl.rows - 1) / group + 1;
+__device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl, const KvSpan& sp, int tile) {
+    int i0 = a.by_group.div(tile * pl.rows), i1 = a.by_group.div(tile * pl.rows + pl.rows - 1) + 1;
     i0 = i0 < sp.lo ? sp.lo : i0;
     i1 = i1 > sp.hi ? sp.hi : i1;
     if (i0 >= i1) return int2{0, 0};
@@ -232,10 +233,15 @@ __device__ __forceinline__ int2 own_records(const KvAttnArgs& a, const Plan& pl,
     return int2{first / KV_GROUP, (sp.start + i1 - 1) / KV_GROUP + 1};
 }
 
-// An entry's place among the items: its records [r0, r1) in `count` chunks of
-// `size` from item `first` on.
+// An entry's place among the items: its records [r0, r1) in `count` chunks from
+// item `first` on.
 struct Cut {
-    int entry, first, count, size, r0, r1;
+    int entry, first, count, r0, r1;
+    KvSpan span;           // of its sequence
+    // where chunk k begins (k = count: the end), the same in every workgroup
+    __device__ __forceinline__ int begin(int k) const {
+        return k >= count ? r1 : r0 + (int)((float)k * ((float)(r1 - r0) * __builtin_amdgcn_rcpf((float)count)));
+    }
 };
 __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
     v += lane_xor1(v);
@@ -247,33 +253,43 @@ __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
 }
 // The cut that holds `item`, or (by_entry) the one of entry `item`; entry -1: an
 // item that no entry needs.  Every wavefront works it out from the lengths in
-// memory: chunks of one size for the whole batch, as small as the items allow,
-// so that long sequences get many workgroups and short ones few.
-__device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int group, int item, bool by_entry) {
-    const uint32_t spare = pl.items - pl.entries;   // > 0
+// memory: one ratio of chunks to records for the whole batch, as high as the
+// items allow, so that long sequences get many workgroups and short ones few.
+// An entry of n records gets floor(n ratio) + 1 chunks: with ratio a little
+// under (items - entries) / records, all of them fit into the items.
+__device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int item, bool by_entry) {
+    const float spare = (float)(pl.items - pl.entries) * (1.f - 0x1p-18f);
+    auto chunks = [&](float ratio, int n) { return n > 0 ? (int)((float)n * ratio) + 1 : 0; };
     if (pl.entries == 1) {
-        const int2 r = own_records(a, pl, 0, 0, group);
+        const KvSpan sp = kv_span(a.rows, a.cache, 0);
+        const int2 r = own_records(a, pl, sp, 0);
         const int n = r.y - r.x;
-        int size = (int)((n + spare - 1) / spare);
-        size = size < pl.least ? pl.least : size;
-        const int count = (n + size - 1) / size;
-        return Cut{by_entry || item < count ? 0 : -1, 0, count, size, r.x, r.y};
+        const int count = chunks(fminf(pl.per_record, spare * __builtin_amdgcn_rcpf((float)n)), n);
+        return Cut{by_entry || item < count ? 0 : -1, 0, count, r.x, r.y, sp};
     }
     const int lane = threadIdx.x & 63;
+    KvSpan sp{0, 0, 0, 0};
     int2 r{0, 0};
-    uint64_t total = 0;
+    auto look = [&](int e) {
+        if (e < pl.entries) {
+            const int b = pl.by_tiles.div(e);
+            sp = kv_span(a.rows, a.cache, b);
+            r = own_records(a, pl, sp, pl.by_tiles.mod(e, b));
+        } else {
+            r = int2{0, 0};
+        }
+    };
+    float total = 0.f;
     for (int e0 = 0; e0 < pl.entries; e0 += 64) {
-        const int e = e0 + lane;
-        r = e < pl.entries ? own_records(a, pl, e / pl.tiles, e % pl.tiles, group) : int2{0, 0};
-        total += wave_sum_u32((uint32_t)(r.y - r.x));   // at most 64 * 2^25
+        look(e0 + lane);
+        total += (float)wave_sum_u32((uint32_t)(r.y - r.x));   // at most 64 * 2^25
     }
-    int size = total >> 32 ? (int)((total + spare - 1) / spare) : (int)(((uint32_t)total + (spare - 1)) / spare);
-    size = size < pl.least ? pl.least : size;
+    const float ratio = fminf(pl.per_record, spare * __builtin_amdgcn_rcpf(total));
     int before = 0;
     for (int e0 = 0; e0 < pl.entries; e0 += 64) {
         const int e = e0 + lane;
-        if (pl.entries > 64) r = e < pl.entries ? own_records(a, pl, e / pl.tiles, e % pl.tiles, group) : int2{0, 0};
-        const int n = (r.y - r.x + size - 1) / size;
+        if (pl.entries > 64) look(e);
+        const int n = chunks(ratio, r.y - r.x);
         int upto = n;
 #pragma unroll
         for (int k = 1; k < 64; k *= 2) {
@@ -284,13 +300,14 @@ __device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int
         const uint64_t who = __ballot(mine);
         if (who) {
             const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)who) - 1);
-            const int count = __builtin_amdgcn_readlane(n, at);
-            return Cut{e0 + at, before + __builtin_amdgcn_readlane(upto, at) - count, count, size,
-                       __builtin_amdgcn_readlane(r.x, at), __builtin_amdgcn_readlane(r.y, at)};
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+            const int count = of(n);
+            return Cut{e0 + at, before + of(upto) - count, count, of(r.x), of(r.y),
+                       KvSpan{of(sp.slot), of(sp.start), of(sp.lo), of(sp.hi)}};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return Cut{-1, 0, 0, size, 0, 0};
+    return Cut{-1, 0, 0, 0, 0, KvSpan{0, 0, 0, 0}};
 }
 
 // Partial results cross XCDs inside a launch (the last workgroup of an entry
@@ -320,7 +337,7 @@ template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE, bool FUSE
 __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl, int wg, float* lds) {
     static_assert(WR * WK == WAVES, "four wavefronts");
     constexpr int HD = NB * 32, ROWS = 16 * R * WR;
-    const int kvh = a.cache.kv_heads, head = wg % kvh, item = wg / kvh, group = a.heads / kvh;
+    const int kvh = a.cache.kv_heads, item = a.by_kv_heads.div(wg), head = wg - item * kvh, group = (int)a.by_group.d;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4;
     const int wr = wave % WR, wk = wave / WR;
 
@@ -337,25 +354,26 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
     } else {
         if (pl.whole) {
             // the longest tiles first, and beside each a short one
-            const int half = (pl.tiles + 1) / 2, k = item / a.rows.batch;
-            b = item % a.rows.batch;
+            const int half = (pl.tiles + 1) / 2, k = pl.by_batch.div(item);
+            b = pl.by_batch.mod(item, k);
             tile = k < half ? pl.tiles - 1 - k : k - half;
-            const int2 r = own_records(a, pl, b, tile, group);
+            sp = kv_span(a.rows, a.cache, b);
+            const int2 r = own_records(a, pl, sp, tile);
             r0 = r.x;
             r1 = r.y;
         } else {
-            const Cut c = find_cut(a, pl, group, item, false);
+            const Cut c = find_cut(a, pl, item, false);
             if (c.entry < 0) return;
             entry = c.entry;
             chunks = c.count;
             first_item = c.first;
-            b = entry / pl.tiles;
-            tile = entry % pl.tiles;
-            r0 = c.r0 + (item - c.first) * c.size;
-            r1 = r0 + c.size < c.r1 ? r0 + c.size : c.r1;
+            b = pl.by_tiles.div(entry);
+            tile = pl.by_tiles.mod(entry, b);
+            r0 = c.begin(item - c.first);
+            r1 = c.begin(item - c.first + 1);
+            sp = c.span;
         }
-        if (r0 >= r1) return;
-        sp = kv_span(a.rows, a.cache, b);
+        if (pl.whole && r0 >= r1) return;
     }
     const KvView& cache = PRE ? a.prefix : a.cache;
     const int slot = PRE ? a.prefix_slot : sp.slot;
@@ -383,18 +401,18 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         KvSpan s = sp;
         bool there;
         if constexpr (PRE) {
-            const int token = row / group;
-            bb = token / tokens;
-            i = token % tokens;
+            const int token = a.by_group.div(row);
+            bb = a.by_tokens.div(token);
+            i = a.by_tokens.mod(token, bb);
             there = bb < a.rows.batch;
             if (there) s = kv_span(a.rows, a.cache, bb);
         } else {
-            i = row / group;
+            i = a.by_group.div(row);
             there = i < tokens;
         }
         there = there && i >= s.lo && i < s.hi;
         const int64_t at = (int64_t)bb * tokens + i;
-        const int h = head * group + row % group;
+        const int h = head * group + (PRE ? a.by_group.mod(row, bb * tokens + i) : a.by_group.mod(row, i));
         out_at[x] = there ? at * a.out_stride + h * HD : -1;
         t[x].init(there ? a.q + at * a.q_stride + h * HD : nullptr, g, a.scale);
         // positions in the cache at hand; an empty row sees all of the chunk
@@ -539,28 +557,40 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         // rows x (HD / 4) lanes, the chunks of a row in as many sets as the threads allow
         constexpr int LANES = HD / 4, SETS = THREADS / LANES;
         const int set = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
-        const int i0 = tile * ROWS / group, i1 = (tile * ROWS + ROWS - 1) / group + 1;
+        const int i0 = a.by_group.div(tile * ROWS), i1 = a.by_group.div(tile * ROWS + ROWS - 1) + 1;
         const int lo = (sp.lo > i0 ? sp.lo : i0) * group, hi = (sp.hi < i1 ? sp.hi : i1) * group;   // its rows
         const int begin = lo > tile * ROWS ? lo - tile * ROWS : 0, end = hi - tile * ROWS < ROWS ? hi - tile * ROWS : ROWS;
         const int rows = end - begin;
-        const int share = SETS / rows > 1 ? SETS / rows : 1;       // sets that split a row's chunks
+        int share = 1;                                     // sets that split a row's chunks
+        while (share * 2 * rows <= SETS) share *= 2;
         auto jo = reinterpret_cast<float (*)[HD]>(lds);
         auto jm = reinterpret_cast<float (*)[2]>(lds + SETS * HD);
-        for (int q0 = 0; q0 < rows; q0 += SETS / share) {
-            const int q = q0 + set / share, part_of = set % share;
-            const bool on = set < SETS / share * share && q < rows;
+        const int at_once = SETS / share, my = set / share, part_of = set % share;
+        for (int q0 = 0; q0 < rows; q0 += at_once) {
+            const int q = q0 + my;
+            const bool on = my < at_once && q < rows;
             float m = -INFINITY, l = 0.f;
             f4 acc{0.f, 0.f, 0.f, 0.f};
             if (on) {
-#pragma unroll 4
-                for (int c = part_of; c < chunks; c += share) {
-                    const int64_t part = ((int64_t)(first_item + c) * kvh + head) * ROWS + begin + q;
-                    const f2 ml = load_past(pl.ml + part * 2);
-                    const f2 oa = load_past(pl.o + part * HD + d), ob = load_past(pl.o + part * HD + d + 2);
-                    float f, w;
-                    join_weights(m, ml[0], f, w);
-                    l = fmaf(l, f, w * ml[1]);
-                    acc = acc * f + f4{oa[0], oa[1], ob[0], ob[1]} * w;
+                constexpr int FLIGHT = 8;                  // chunks whose loads are out together
+                for (int c0 = part_of; c0 < chunks; c0 += FLIGHT * share) {
+                    f2 ml[FLIGHT], oa[FLIGHT], ob[FLIGHT];
+#pragma unroll
+                    for (int z = 0; z < FLIGHT; z++) {
+                        const int c = c0 + z * share < chunks ? c0 + z * share : c0;
+                        const int64_t part = ((int64_t)(first_item + c) * kvh + head) * ROWS + begin + q;
+                        ml[z] = load_past(pl.ml + part * 2);
+                        oa[z] = load_past(pl.o + part * HD + d);
+                        ob[z] = load_past(pl.o + part * HD + d + 2);
+                    }
+#pragma unroll
+                    for (int z = 0; z < FLIGHT; z++) {
+                        if (c0 + z * share >= chunks) break;
+                        float f, w;
+                        join_weights(m, ml[z][0], f, w);
+                        l = fmaf(l, f, w * ml[z][1]);
+                        acc = acc * f + f4{oa[z][0], oa[z][1], ob[z][0], ob[z][1]} * w;
+                    }
                 }
                 *reinterpret_cast<f4*>(&jo[set][d]) = acc;
                 if (d == 0) { jm[set][0] = m; jm[set][1] = l; }
@@ -573,8 +603,8 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
                     l = fmaf(l, f, w * jm[set + c][1]);
                     acc = acc * f + *reinterpret_cast<const f4*>(&jo[set + c][d]) * w;
                 }
-                const int row = tile * ROWS + begin + q;
-                const int64_t at = ((int64_t)b * tokens + row / group) * a.out_stride + (head * group + row % group) * HD;
+                const int row = tile * ROWS + begin + q, i = a.by_group.div(row);
+                const int64_t at = ((int64_t)b * tokens + i) * a.out_stride + (head * group + a.by_group.mod(row, i)) * HD;
                 *reinterpret_cast<f4*>(a.out + at + d) = acc * (1.f / l);
             }
             __syncthreads();
@@ -600,15 +630,17 @@ __global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
 // hd / 4 lanes to a chunk and as many chunks at a time as fit; the order of the
 // sums depends on their number alone.
 __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan own, Plan pre) {
-    const int kvh = a.cache.kv_heads, group = a.heads / kvh, hd = a.cache.head_dim;
-    const int h = blockIdx.x % a.heads, token = blockIdx.x / a.heads;
-    const int b = token / a.rows.tokens, i = token % a.rows.tokens, head = h / group, hr = h % group;
+    const int kvh = a.cache.kv_heads, group = (int)a.by_group.d, hd = a.cache.head_dim;
+    // rows of a token: kv head by kv head
+    const int x = a.by_group.div(blockIdx.x), hr = a.by_group.mod(blockIdx.x, x), token = a.by_kv_heads.div(x),
+              head = a.by_kv_heads.mod(x, token), h = head * group + hr;
+    const int b = a.by_tokens.div(token), i = a.by_tokens.mod(token, b);
     const KvSpan sp = kv_span(a.rows, a.cache, b);
     if (i < sp.lo || i >= sp.hi) return;
     const int row = i * group + hr, tile = row / own.rows, trow = row % own.rows;
-    Cut c{0, 0, 1, 0, 0, 0};
+    Cut c{0, 0, 1, 0, 0, sp};
     if (!own.whole) {
-        c = find_cut(a, own, group, b * own.tiles + tile, true);
+        c = find_cut(a, own, b * own.tiles + tile, true);
     } else {   // the item that takes the entry
         const int half = (own.tiles + 1) / 2;
         c.first = (tile >= own.tiles - half ? own.tiles - 1 - tile : tile + half) * a.rows.batch + b;
@@ -659,6 +691,7 @@ struct Config {
 };
 constexpr int PRE_R = 2;
 constexpr int TARGET = 512;        // workgroups: two per CU
+constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (25.0 us against 27.6 at 512)
 constexpr size_t ARRIVED_BYTES = 4 * 2 * TARGET;   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
@@ -687,7 +720,11 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
     o.rows = 16 * p.own_cfg.r * p.own_cfg.wr;
     o.tiles = tiles_of(rows, o.rows);
     o.entries = batch * o.tiles;
-    o.least = p.own_cfg.wk;
+    // two records a wavefront pay for a chunk's own time (4096 keys of the 7B shape: 10.8 us, at one 12.6)
+    o.least = 2 * p.own_cfg.wk;
+    o.per_record = 1.f / (float)o.least * (1.f - 0x1p-18f);
+    o.by_tiles = Divisor(o.tiles);
+    o.by_batch = Divisor(batch);
     const int64_t most = tiles_of(c.groups, o.least);   // chunks of an entry
     o.items = o.entries;
     if (p.own_cfg.wk > 1 && o.entries < want && most > 1) o.items += (int)std::min(want, o.entries * most);
@@ -711,7 +748,8 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
         x.rows = 16 * std::min(PRE_R, r);
         x.tiles = x.entries = tiles_of(batch * rows, x.rows);
         x.least = 4;
-        int64_t chunks = x.entries < want ? want / x.entries : 1;
+        const int64_t most_pre = PRE_TARGET / c.kv_heads;
+        int64_t chunks = x.entries < most_pre ? most_pre / x.entries : 1;
         if (prefix_len >= 0) chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, tiles_of(prefix_len, KV_GROUP) / x.least));
         x.items = (int)(x.entries * chunks);
         take_parts(x);
@@ -733,7 +771,10 @@ void launch_own(const Plans& p, const KvAttnArgs& a, hipStream_t s) {
 }
 
 template <int NB, bool KQ4, bool VQ4>
-hipError_t launch_types(const KvAttnArgs& a, hipStream_t s) {
+hipError_t launch_types(KvAttnArgs a, hipStream_t s) {
+    a.by_group = Divisor(a.heads / a.cache.kv_heads);
+    a.by_tokens = Divisor(a.rows.tokens);
+    a.by_kv_heads = Divisor(a.cache.kv_heads);
     const Plans p = make_plans(a.cache, a.heads, a.rows.batch, a.rows.tokens, a.prefix_len > 0, a.prefix_len, a.work);
     if (p.pre.items) launch_own<NB, KQ4, VQ4, NB == 8 ? 1 : PRE_R>(p, a, s);
     else launch_own<NB, KQ4, VQ4, 0>(p, a, s);

@@ -47,6 +47,22 @@ __host__ __device__ constexpr int kv_v_byte(bool q4, int p, int r) {
 }
 __host__ __device__ constexpr int kv_v_high(int r) { return r >> 4; }
 
+// Division by a number that the host knows: n / d for 0 <= n < 2^31, with
+// 2^(l-1) < d <= 2^l and m = floor(2^32 (2^l - d) / d) + 1 (Granlund and
+// Montgomery's invariant division).
+struct Divisor {
+    uint32_t d, m, l;
+    Divisor() = default;
+    explicit Divisor(int v) : d((uint32_t)v), m(0), l(0) {
+        while (l < 31 && ((uint32_t)1 << l) < d) l++;
+        m = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> l);
+    }
+    __device__ __forceinline__ int mod(int n, int quotient) const { return n - quotient * (int)d; }
+};
+
 struct KvView {
     uint8_t *k, *v;             // [slots][kv_heads][groups] records
     int slots, kv_heads, head_dim, capacity, groups;
