@@ -198,6 +198,23 @@ def check(rc: int) -> None:
         raise HipError(rc, msg.decode("utf-8", "replace") if msg else "unknown error")
 
 
+# The reference's exception types for the status codes that have one.
+_EXC = {E_INVALID: ValueError, E_UNSUPPORTED: NotImplementedError, E_NOT_FOUND: KeyError, E_RANGE: IndexError}
+
+
+def call(rc: int) -> None:
+    """check, with the exceptions that the reference throws for the same condition."""
+    if rc == OK:
+        return
+    try:
+        check(rc)
+    except HipError as e:
+        exc = _EXC.get(e.code)
+        if exc is not None:
+            raise exc(str(e)) from None
+        raise
+
+
 def ptr(a) -> C.c_void_p | None:
     """Host pointer of a C-contiguous numpy array (None for None)."""
     if a is None:

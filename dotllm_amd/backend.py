@@ -21,21 +21,9 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import check, lib, ptr
-
-_EXC = {_lib.E_INVALID: ValueError, _lib.E_UNSUPPORTED: NotImplementedError,
-        _lib.E_NOT_FOUND: KeyError, _lib.E_RANGE: IndexError}
-
-
-def _call(rc: int) -> None:
-    try:
-        check(rc)
-    except _lib.HipError as e:
-        exc = _EXC.get(e.code)
-        if exc is not None:
-            raise exc(str(e)) from None
-        raise
-
+from ._lib import call as _call
+from ._lib import lib, ptr
+from .device import DeviceArray, address
 
 def _f32(a, name: str) -> np.ndarray:
     if not (isinstance(a, np.ndarray) and a.dtype == np.float32 and a.flags["C_CONTIGUOUS"]):
@@ -56,6 +44,16 @@ def sampling_struct(options) -> "_lib.Sampling":
                     float(options.repeat_penalty), int(options.repeat_penalty_window_size))
 
 
+class Place:
+    """Where a backend's memory is, as arrays of other owners say it."""
+
+    def __init__(self, index: int):
+        self.type, self.index = "cuda", index
+
+    def __repr__(self):
+        return f"{self.type}:{self.index}"
+
+
 class HipBackend:
     """IComputeBackend over one MI355X device (context + stream + weight cache)."""
 
@@ -63,6 +61,7 @@ class HipBackend:
         self._ctx = C.c_void_p()
         _call(lib().llmdot_hip_create(device, C.byref(self._ctx)))
         self.device = device
+        self.place = Place(device)
 
     # -- IDisposable -------------------------------------------------------
     def dispose(self) -> None:
@@ -220,7 +219,6 @@ class HipBackend:
 
     def verify_workspace(self, batch: int, drafts: int, vocab: int):
         """Device memory that suffices for verify_drafts calls of that size."""
-        from .device import DeviceArray
         n = C.c_size_t(0)
         _call(lib().llmdot_hip_verify_drafts_workspace(self._ctx, batch, drafts, vocab, C.byref(n)))
         return DeviceArray(self, (n.value,), "uint8")
@@ -234,7 +232,6 @@ class HipBackend:
         drafts that came with certainty), counts [batch] int32 (None: n each).  tokens_out
         [batch, n + 1]: the standing drafts, the next token, then -1; accepted_out [batch]: how
         many stand.  All arrays in device memory; temperature <= 0 is greedy."""
-        from .device import address
         dev = self.device
         b, n1, vocab = target.shape
         n = n1 - 1
@@ -294,3 +291,4 @@ class HipBackend:
         if inp.size < need or weights.size < need or output.size < input_dim:
             raise IndexError("input and weights must hold kernelSize * inputDim elements, output inputDim")
         _call(lib().llmdot_hip_conv1d(self._ctx, ptr(inp), ptr(weights), ptr(output), kernel_size, input_dim))
+

@@ -86,7 +86,7 @@ __device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const h2 h = __builtin_convertvector(f2{x[i], x[i + 1]}, h2);
-        const h2 l = __builtin_convertvector(f2{x[i] - (float)h[0], x[i + 1] - (float)h[1]}, h2);
+        const h2 l = __builtin_convertvector(f2{fmaf((float)h[0], -1.f, x[i]), fmaf((float)h[1], -1.f, x[i + 1])}, h2);
         hi[i] = h[0]; hi[i + 1] = h[1];
         lo[i] = l[0]; lo[i + 1] = l[1];
     }
@@ -335,14 +335,14 @@ __device__ __forceinline__ void join_weights(float& m, float mk, float& f, float
 // workgroup that finishes an entry's last chunk joins them.
 template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE, bool FUSE>
 __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl, int wg, float* lds) {
-    static_assert(WR * WK == WAVES, "four wavefronts");
+    static_assert(WR * WK == WAVES, "four wavefronts to a tile");
     constexpr int HD = NB * 32, ROWS = 16 * R * WR;
     const int kvh = a.cache.kv_heads, item = a.by_kv_heads.div(wg), head = wg - item * kvh, group = (int)a.by_group.d;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4;
-    const int wr = wave % WR, wk = wave / WR;
+    const int wr = wave % WR, wk = wave / WR % WK;
 
     // which rows and records
-    int b = 0, tile, r0, r1, entry = 0, chunks = 1, first_item = item;
+    int b = 0, tile, r0, r1, entry = 0, chunks = 1, first_item = 0, at_item = item;   // at_item: place in the workspace
     KvSpan sp{0, 0, 0, 0};
     if constexpr (PRE) {
         const int per = pl.items / pl.entries, total = (a.prefix_len + KV_GROUP - 1) / KV_GROUP;
@@ -353,10 +353,16 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         r1 = low + (int)((int64_t)n * (k + 1) / per);
     } else {
         if (pl.whole) {
-            // the longest tiles first, and beside each a short one
-            const int half = (pl.tiles + 1) / 2, k = pl.by_batch.div(item);
+            // the longest tiles first; with keys to a wavefront (WK = 1), the long
+            // tile's four wavefronts share the SIMDs with a short one's
+            const int k = pl.by_batch.div(item);
             b = pl.by_batch.mod(item, k);
-            tile = k < half ? pl.tiles - 1 - k : k - half;
+            tile = pl.tiles - 1 - k;
+            if (WK == 1 && wave >= WAVES) {
+                if (k == tile) return;
+                tile = k;
+            }
+            at_item = b * pl.tiles + tile;
             sp = kv_span(a.rows, a.cache, b);
             const int2 r = own_records(a, pl, sp, tile);
             r0 = r.x;
@@ -498,7 +504,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
                 f[w] = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
                 sum = fmaf(f[w], sm[wr + w * WR][row][1], sum);
             }
-            const int64_t part = ((int64_t)item * kvh + head) * ROWS + wr * R * 16 + row;
+            const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + wr * R * 16 + row;
             const float inv = 1.f / sum;
             if (out_at[x] < 0) continue;
             for (int d = wk; d < 2 * NB; d += WK) {
@@ -532,7 +538,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
                     *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = t[x].o[d] * inv;
             } else {
                 const int trow = (wr * R + x) * 16 + (lane & 15);
-                const int64_t part = ((int64_t)item * kvh + head) * ROWS + trow;
+                const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + trow;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = t[x].o[d];
                 if (g == 0) *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{t[x].m, t[x].l};
@@ -614,9 +620,11 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
 
 // The call's own chunks, and (RP) the prefix's before them, 16 RP rows to a wavefront.
 template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, int RP>
-__global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(KvAttnArgs a, Plan own, Plan pre) {
+__global__ __launch_bounds__(WK == 1 ? 2 * THREADS : THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
+    KvAttnArgs a, Plan own, Plan pre) {
     constexpr int MOST = RP > (WK > 1 ? R : 0) ? RP : WK > 1 ? R : 0;   // tiles of a wavefront that meet in LDS
     __shared__ __align__(16) float lds[MOST > 0 ? WAVES * 16 * MOST * (NB * 32 + 6) + 4 : 4];
+    static_assert(RP == 0 || WK > 1, "the prefix's chunks take four wavefronts");
     if constexpr (RP > 0) {
         const int before = pre.items * a.cache.kv_heads;
         if ((int)blockIdx.x < before) attend_chunk<NB, KQ4, VQ4, RP, 1, 4, true, false>(a, pre, blockIdx.x, lds);
@@ -641,9 +649,8 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     Cut c{0, 0, 1, 0, 0, sp};
     if (!own.whole) {
         c = find_cut(a, own, b * own.tiles + tile, true);
-    } else {   // the item that takes the entry
-        const int half = (own.tiles + 1) / 2;
-        c.first = (tile >= own.tiles - half ? own.tiles - 1 - tile : tile + half) * a.rows.batch + b;
+    } else {
+        c.first = b * own.tiles + tile;
     }
     const int prow = token * group + hr;
     const int pchunks = pre.items ? pre.items / pre.entries : 0, ptile = pre.items ? prow / pre.rows : 0;
@@ -697,6 +704,7 @@ constexpr size_t ARRIVED_BYTES = 4 * 2 * TARGET;   // entries * kv_heads <= TARG
 struct Plans {
     Config own_cfg;
     Plan own{}, pre{};
+    int groups;            // workgroups of the own part, per kv head
     bool fused;
     size_t bytes = 0;
 };
@@ -705,16 +713,18 @@ int rows_per_wave(int blocks) { return blocks == 8 ? 1 : 2; }   // tiles of 16: 
 
 // Shapes of the launch, from sizes that the host knows (lengths are on the
 // device).  16 rows or fewer (decode): four wavefronts share the keys of one
-// tile.  More: four wavefronts of 32 rows each over the same keys where that
-// gives a workgroup for every CU, else one such tile per workgroup, its keys
-// over the wavefronts and, in chunks, over workgroups.
+// tile.  More: one tile of 32 rows per workgroup, its keys over the wavefronts
+// and, in chunks, over workgroups; where prompts are so long that pairs of 128
+// rows give a workgroup for every CU, four wavefronts of 32 rows each walk the
+// same keys (not at head_dim 256, whose tiles leave no registers for two
+// wavefronts per SIMD).
 Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len, uint8_t* work) {
     Plans p;
     const int group = heads / c.kv_heads, r = rows_per_wave(c.head_dim / 32);
     const int64_t rows = (int64_t)tokens * group, want = TARGET / c.kv_heads;
     auto tiles_of = [](int64_t n, int per) { return (int)((n + per - 1) / per); };
     if (rows <= 16) p.own_cfg = {1, 1, 4};
-    else if ((int64_t)batch * tiles_of(rows, 64 * r) * c.kv_heads >= TARGET / 2) p.own_cfg = {r, 4, 1};
+    else if (!prefix && r == 2 && (int64_t)batch * tiles_of(rows, 128 * r) * c.kv_heads >= TARGET / 2) p.own_cfg = {r, 4, 1};
     else p.own_cfg = {r, 1, 4};
     Plan& o = p.own;
     o.rows = 16 * p.own_cfg.r * p.own_cfg.wr;
@@ -727,7 +737,9 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
     o.by_batch = Divisor(batch);
     const int64_t most = tiles_of(c.groups, o.least);   // chunks of an entry
     o.items = o.entries;
-    if (p.own_cfg.wk > 1 && o.entries < want && most > 1) o.items += (int)std::min(want, o.entries * most);
+    if (p.own_cfg.wk > 1 && o.entries < want && most > 1)
+        o.items = (int)std::max<int64_t>(std::min(want, o.entries * (most + 1)), o.entries * 3 / 2 + 1);
+    p.groups = p.own_cfg.wk > 1 ? o.items : batch * tiles_of(o.tiles, 2);
     o.whole = o.items == o.entries ? prefix ? 2 : 1 : 0;
     p.fused = !prefix && p.own_cfg.r == 1 && p.own_cfg.wk == 4 && !o.whole;
     size_t at = 0;
@@ -761,13 +773,13 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
 
 template <int NB, bool KQ4, bool VQ4, int RP>
 void launch_own(const Plans& p, const KvAttnArgs& a, hipStream_t s) {
-    const dim3 grid((uint32_t)((p.own.items + p.pre.items) * a.cache.kv_heads));
+    const dim3 grid((uint32_t)((p.groups + p.pre.items) * a.cache.kv_heads));
     constexpr int R = NB == 8 ? 1 : 2;
     const Config& f = p.own_cfg;
     if (a.rows.tokens * (a.heads / a.cache.kv_heads) <= 16)
         kv_attention_kernel<NB, KQ4, VQ4, 1, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
     else if (f.wr == 1) kv_attention_kernel<NB, KQ4, VQ4, R, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
-    else kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
+    else if constexpr (RP == 0 && R == 2) kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, 0><<<grid, 2 * THREADS, 0, s>>>(a, p.own, p.pre);
 }
 
 template <int NB, bool KQ4, bool VQ4>

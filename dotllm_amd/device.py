@@ -14,8 +14,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import lib, ptr
-from .backend import HipBackend, _call
+from ._lib import call, lib, ptr
 
 _TYPES = {"float32": "<f4", "int32": "<i4"}
 
@@ -23,17 +22,17 @@ _TYPES = {"float32": "<f4", "int32": "<i4"}
 class DeviceArray:
     """Zeroed memory of a backend's device, freed with the array."""
 
-    def __init__(self, backend: HipBackend, shape, dtype="float32"):
+    def __init__(self, backend: "HipBackend", shape, dtype="float32"):
         self.backend = backend
         self.shape = tuple(int(n) for n in (shape if hasattr(shape, "__len__") else (shape,)))
         self.dtype = np.dtype(dtype)
         self.size = int(np.prod(self.shape, dtype=np.int64))
         self.nbytes = self.size * self.dtype.itemsize
         self._p = C.c_void_p()
-        _call(lib().llmdot_hip_device_alloc(backend.handle, max(self.nbytes, 16), C.byref(self._p)))
+        call(lib().llmdot_hip_device_alloc(backend.handle, max(self.nbytes, 16), C.byref(self._p)))
 
     @classmethod
-    def of(cls, backend: HipBackend, values, dtype=None) -> "DeviceArray":
+    def of(cls, backend: "HipBackend", values, dtype=None) -> "DeviceArray":
         """A copy of host values."""
         a = np.ascontiguousarray(values, dtype=dtype)
         out = cls(backend, a.shape, a.dtype)
@@ -46,17 +45,24 @@ class DeviceArray:
         if a.size != self.size:
             raise ValueError(f"{a.size} values for an array of {self.size}")
         if a.nbytes:
-            _call(lib().llmdot_hip_memcpy_h2d(self.backend.handle, self._p, ptr(a), a.nbytes))
+            call(lib().llmdot_hip_memcpy_h2d(self.backend.handle, self._p, ptr(a), a.nbytes))
 
     def get(self) -> np.ndarray:
         """The values on the host, after everything the backend's stream holds."""
         a = np.empty(self.shape, dtype=self.dtype)
         if a.nbytes:
-            _call(lib().llmdot_hip_memcpy_d2h(self.backend.handle, ptr(a), self._p, a.nbytes))
+            call(lib().llmdot_hip_memcpy_d2h(self.backend.handle, ptr(a), self._p, a.nbytes))
         return a
+
+    @property
+    def device(self) -> "Place":
+        return self.backend.place
 
     def data_ptr(self) -> int:
         return self._p.value
+
+    def is_contiguous(self) -> bool:
+        return True
 
     @property
     def __cuda_array_interface__(self) -> dict:
@@ -75,23 +81,15 @@ class DeviceArray:
             pass
 
 
+_NAMES = {"float32": ("float32", "torch.float32"), "int32": ("int32", "torch.int32")}
+
+
 def address(a, name: str, dtype: str, shape: tuple, device: int) -> int:
     """The address of a contiguous device array of the given type and shape."""
     where = getattr(a, "data_ptr", None)
     if where is not None:
-        kind = str(a.dtype)
-        if not (kind == dtype or kind == "torch." + dtype):
-            raise ValueError(f"{name} must be {dtype}, not {kind}")
-        if tuple(a.shape) != shape:
-            raise ValueError(f"{name} must have shape {shape}, not {tuple(a.shape)}")
-        if not isinstance(a, DeviceArray):
-            at = a.device
-            if at.type != "cuda" or at.index != device:
-                raise ValueError(f"{name} is on {at}, not on device {device}")
-            if not a.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
-        elif a.backend.device != device:
-            raise ValueError(f"{name} is on device {a.backend.device}, not on {device}")
+        if a.device.index != device or a.shape != shape or str(a.dtype) not in _NAMES[dtype] or not a.is_contiguous():
+            _refuse(a, name, dtype, shape, device)
         return where()
     face = getattr(a, "__cuda_array_interface__", None)
     if face is None:
@@ -111,12 +109,24 @@ def address(a, name: str, dtype: str, shape: tuple, device: int) -> int:
     return face["data"][0]
 
 
+def _refuse(a, name: str, dtype: str, shape: tuple, device: int) -> None:
+    if a.device.index != device:   # host arrays have no index
+        raise ValueError(f"{name} is on {a.device}, not on device {device}")
+    if tuple(a.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(a.shape)}")
+    if str(a.dtype) not in _NAMES[dtype]:
+        raise ValueError(f"{name} must be {dtype}, not {a.dtype}")
+    raise ValueError(f"{name} must be contiguous")
+
+
 def rows(a, name: str, shape: tuple, device: int) -> tuple:
     """Address and row stride (floats) of a float32 array [batch, tokens, heads, head_dim] whose
     rows are whole and equally far apart: contiguous, or a slice of wider rows (a fused projection's)."""
     stride = getattr(a, "stride", None)
-    if stride is None or tuple(a.shape) != shape or a.is_contiguous():
+    if stride is None or a.is_contiguous():
         return address(a, name, "float32", shape, device), 0
+    if a.device.index != device or a.shape != shape or str(a.dtype) not in _NAMES["float32"]:
+        _refuse(a, name, "float32", shape, device)
     b, t, h, d = shape
     sb, st, sh, sd = stride()
     if 0 in shape or sd != 1 or (h > 1 and sh != d):
@@ -124,6 +134,4 @@ def rows(a, name: str, shape: tuple, device: int) -> tuple:
     step = st if t > 1 else sb if b > 1 else 0
     if b > 1 and t > 1 and sb != t * st:
         raise ValueError(f"{name}'s rows must be equally far apart")
-    if str(a.dtype) != "torch.float32" or a.device.type != "cuda" or a.device.index != device:
-        raise ValueError(f"{name} must be float32 on device {device}, not {a.dtype} on {a.device}")
     return a.data_ptr(), step

@@ -19,8 +19,8 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from ._lib import Q8_0, lib
-from .backend import HipBackend, _call
+from ._lib import Q8_0, call, lib
+from .backend import HipBackend
 from .device import DeviceArray, address, rows
 
 
@@ -30,6 +30,7 @@ class TokenBatch:
     def __init__(self, sequences: int, tokens: int, arrays: tuple, addresses: tuple):
         self.sequences, self.tokens, self._arrays = sequences, tokens, arrays
         self.struct = _lib.TokenBatch(sequences, tokens, *addresses)
+        self.ref = C.byref(self.struct)
 
 
 class KvCache:
@@ -40,7 +41,8 @@ class KvCache:
         self.slots, self.kv_heads, self.head_dim, self.capacity = slots, kv_heads, head_dim, capacity
         self.k_type, self.v_type = k_type, v_type
         d = _lib.KvCacheDesc(slots, kv_heads, head_dim, capacity, k_type, v_type)
-        _call(lib().llmdot_hip_kv_cache_create(backend.handle, C.byref(d), C.byref(self._c)))
+        self._lib = lib()
+        call(self._lib.llmdot_hip_kv_cache_create(backend.handle, C.byref(d), C.byref(self._c)))
 
     def dispose(self) -> None:
         if self._c:
@@ -82,19 +84,19 @@ class KvCache:
         shape = (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
         kp, ks = rows(k, "k", shape, self.backend.device)
         vp, vs = rows(v, "v", shape, self.backend.device)
-        _call(lib().llmdot_hip_kv_cache_write(self.handle, kp, ks, vp, vs, C.byref(batch.struct)))
+        call(self._lib.llmdot_hip_kv_cache_write(self.handle, kp, ks, vp, vs, batch.ref))
 
     def read(self, k_out, v_out, batch: TokenBatch) -> None:
         """What the cache holds at the batch's positions, as fp32; other rows stay as they are."""
         shape = (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
         kp, ks = rows(k_out, "k_out", shape, self.backend.device)
         vp, vs = rows(v_out, "v_out", shape, self.backend.device)
-        _call(lib().llmdot_hip_kv_cache_read(self.handle, kp, ks, vp, vs, C.byref(batch.struct)))
+        call(self._lib.llmdot_hip_kv_cache_read(self.handle, kp, ks, vp, vs, batch.ref))
 
     def attention_workspace(self, heads: int, sequences: int, tokens: int, prefix: bool = False) -> DeviceArray:
         """Device memory that suffices for attention calls of that size."""
         n = C.c_size_t(0)
-        _call(lib().llmdot_hip_kv_cache_attention_workspace(self.handle, heads, sequences, tokens, int(prefix),
+        call(lib().llmdot_hip_kv_cache_attention_workspace(self.handle, heads, sequences, tokens, int(prefix),
                                                             C.byref(n)))
         return DeviceArray(self.backend, (n.value,), "uint8")
 
@@ -104,10 +106,10 @@ class KvCache:
         [sequences, tokens, heads, head_dim].  Rows 0 .. prefix_len - 1 of slot `prefix_slot` of
         `prefix` come before every sequence's own; window > 0 keeps the last `window` positions;
         scale 0 is 1 / sqrt(head_dim).  Rows past a sequence's count stay as they are."""
-        shape = (batch.sequences, batch.tokens, int(q.shape[2]) if len(q.shape) == 4 else 0, self.head_dim)
+        shape = (batch.sequences, batch.tokens, q.shape[2] if len(q.shape) == 4 else 0, self.head_dim)
         qp, qs = rows(q, "q", shape, self.backend.device)
         op, os_ = rows(out, "out", shape, self.backend.device)
         opt = _lib.Attention(shape[2], window, scale, prefix.handle if prefix is not None else None, prefix_slot,
                              prefix_len, qs, os_)
-        _call(lib().llmdot_hip_kv_cache_attention(self.handle, qp, op, C.byref(batch.struct), C.byref(opt),
-                                                  workspace.data_ptr(), workspace.nbytes))
+        call(self._lib.llmdot_hip_kv_cache_attention(self.handle, qp, op, batch.ref, C.byref(opt), workspace.data_ptr(),
+                                                      workspace.nbytes))
