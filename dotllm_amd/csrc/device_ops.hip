@@ -257,9 +257,9 @@ extern "C" int32_t llmdot_hip_kv_cache_attention(llmdot_hip_kv_cache* cache, con
 namespace {
 int check_verify_shape(int batch, int drafts, int vocab) {
     if (batch < 0 || drafts < 0 || vocab <= 0) return ctx_fail(LLMDOT_E_INVALID, "bad batch, drafts or vocabulary");
-    if (batch > 65535 || drafts > 1024 || vocab > (1 << 24))
-        return ctx_fail(LLMDOT_E_UNSUPPORTED, "at most 65535 sequences, 1024 drafts and 2^24 tokens in a vocabulary");
-    if ((int64_t)batch * (vocab / 2048 + 1) > MAX_GRID) return ctx_fail(LLMDOT_E_UNSUPPORTED, "too many logits in a call");
+    if (batch > VERIFY_BATCH || drafts > 1024 || vocab > (1 << 24))
+        return ctx_fail(LLMDOT_E_UNSUPPORTED, "at most 4096 sequences, 1024 drafts and 2^24 tokens in a vocabulary");
+    if ((int64_t)batch * (vocab / 1024 + 1) > MAX_GRID) return ctx_fail(LLMDOT_E_UNSUPPORTED, "too many logits in a call");
     return 0;
 }
 }  // namespace
@@ -296,7 +296,7 @@ extern "C" int32_t llmdot_hip_verify_drafts(llmdot_hip_ctx* ctx, const float* ta
                                                       std::to_string(need));
         }
         VerifyArgs a{target_dev, draft_dev, drafts_dev, counts_dev, uniforms_dev, batch, drafts, vocab, temperature,
-                     tokens_dev, accepted_dev, static_cast<uint8_t*>(workspace_dev)};
+                     tokens_dev, accepted_dev, static_cast<uint8_t*>(workspace_dev), 0.0, 0.0};
         OnDevice dev(ctx_device(ctx));
         hipError_t e = dev.err;
         if (e == hipSuccess) e = launch_verify(a, ctx_stream(ctx));

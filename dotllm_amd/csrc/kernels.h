@@ -301,6 +301,10 @@ hipError_t launch_prefill_attn_wave(const PfAttnArgs& a, hipStream_t s);
 hipError_t launch_embed_rows(const uint8_t* table, uint32_t type, int hidden, const int32_t* tokens, int T, float* out,
                              hipStream_t s);
 
+// Words between two arrival counters of a launch: atomics on one line of memory
+// wait for each other (about 14 ns each, whichever counter they are for).
+constexpr int COUNTER_STRIDE = 32;
+
 // ---- kv_cache.hip, kv_attention.hip (quantised KV cache) ----
 // Rows of k and v [batch * tokens], ks and vs floats apart, into the cache, and back.
 hipError_t launch_kv_write(const KvView& c, const KvRows& rows, const float* k, int64_t ks, const float* v, int64_t vs,
@@ -324,6 +328,7 @@ size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens,
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s);
 
 // ---- verify.hip (verification of drafted tokens) ----
+constexpr int VERIFY_BATCH = 4096;   // sequences of a call, at most
 struct VerifyArgs {
     const float *target, *draft;    // [batch][drafts + 1][vocab], [batch][drafts][vocab] or null
     const int32_t *draft_tokens, *counts;
@@ -332,8 +337,9 @@ struct VerifyArgs {
     float temperature;
     int32_t *tokens_out, *accepted_out;
     uint8_t* work;                  // verify_workspace bytes
+    double rate, reach;             // log2(e) / temperature, and 1000 over it (set by the launcher)
 };
 size_t verify_workspace(int batch, int drafts, int vocab);
-hipError_t launch_verify(const VerifyArgs& a, hipStream_t s);
+hipError_t launch_verify(VerifyArgs a, hipStream_t s);
 
 }  // namespace llmdot

@@ -553,7 +553,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         int& is_last = *reinterpret_cast<int*>(lds + WAVES * 16 * R * (HD + 6));
         __syncthreads();
         if (threadIdx.x == 0) {
-            uint32_t* count = pl.arrived + entry * kvh + head;
+            uint32_t* count = pl.arrived + (entry * kvh + head) * COUNTER_STRIDE;
             const uint32_t was = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             is_last = was + 1 == (uint32_t)chunks;
             if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -699,7 +699,7 @@ struct Config {
 constexpr int PRE_R = 2;
 constexpr int TARGET = 512;        // workgroups: two per CU
 constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (25.0 us against 27.6 at 512)
-constexpr size_t ARRIVED_BYTES = 4 * 2 * TARGET;   // entries * kv_heads <= TARGET where chunks are counted
+constexpr size_t ARRIVED_BYTES = (size_t)4 * TARGET * COUNTER_STRIDE;   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
     Config own_cfg;

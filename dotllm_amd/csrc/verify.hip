@@ -8,11 +8,12 @@
 // the sums would otherwise decide draws next to one of the 2 V borders (a 32-bit
 // cumulative sum over 128k tokens puts some 2% of the draws next to one).
 //
-// Three launches, each over slices of 2048 logits so that a single sequence
+// Two launches, each over slices of 1024 or 4096 logits so that a single sequence
 // fills the card: maximum and mass of every row's slices (the only pass over all
-// rows); the drafts decided, by every workgroup for itself, and the residual's
-// mass in the slices of the one row that matters; the slice that holds the
-// draw, scanned.
+// rows); then every workgroup decides its sequence's drafts for itself and sums
+// the residual in its slice of the one row that matters, and the last of them
+// finds the slice that holds the draw and scans it.  Bound by reading the logits
+// and, about as long, by the 64-bit exponentials.
 #include "kernels.h"
 #include "common.h"
 
@@ -23,8 +24,8 @@ namespace llmdot {
 namespace {
 
 constexpr int VT = 256;              // threads
-constexpr int PER = 8;               // logits per thread
-constexpr int SLICE = VT * PER;
+constexpr int WAVES = VT / 64;
+constexpr int QUAD = 4;              // consecutive logits of a thread; quads of a slice lie VT * QUAD apart
 
 // Maximum and mass of a slice (greedy: the maximum's first index).
 struct SliceStats {
@@ -45,40 +46,62 @@ struct SliceMass {
     double r, p;           // residual, and the target's own mass
 };
 struct Work {              // in the workspace
+    float* picked;         // [batch][rows] logit of each row's drafted token
+    uint32_t* drawn;       // [VERIFY_BATCH] workgroups done with a sequence, zero between launches
     SliceStats* stats;     // [batch][rows][slices], target rows first
-    Verdict* verdict;      // [batch]
     SliceMass* mass;       // [batch][slices]
     int rows, slices;
 };
 
-// 2^y for y <= 0 by its Taylor series about the nearest integer (12 terms:
-// 2e-16 of the value for |f| <= 1/2); y under -1200 and NaN give 0.
-__device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -1200.0);
-    const double k = rint(y), f = y - k;
-    double r = 2.5678435993488206e-11;                       // ln2^12 / 12!
-    r = fma(r, f, 4.4455382718708116e-10);
-    r = fma(r, f, 7.0549116208011234e-09);
-    r = fma(r, f, 1.0178086009239699e-07);
-    r = fma(r, f, 1.3215486790144309e-06);
-    r = fma(r, f, 1.5252733804059841e-05);
-    r = fma(r, f, 1.5403530393381608e-04);
-    r = fma(r, f, 1.3333558146428443e-03);
-    r = fma(r, f, 9.6181291076284772e-03);
-    r = fma(r, f, 5.5504108664821580e-02);
-    r = fma(r, f, 2.4022650695910071e-01);
-    r = fma(r, f, 6.9314718055994531e-01);
-    r = fma(r, f, 1.0);
-    return ldexp(r, (int)k);
-}
-
-// exp((x - mx) / T), c = log2(e) / T; NaN has no mass, and where the maximum is
-// +infinity only the infinities have some.
-__device__ __forceinline__ double mass(float x, float mx, double c) {
-    if (mx == INFINITY) return x == INFINITY ? 1.0 : 0.0;
-    return exp2_64(((double)x - (double)mx) * c);
-}
-__device__ __forceinline__ double rate(double temperature) { return 1.4426950408889634074 / temperature; }
+// exp((x - mx) / T) for the logits x of a row with maximum mx.  2^y with y =
+// (x - mx) log2(e) / T: the nearest integer goes into the exponent, the rest
+// (|f| <= 1/2) through the Taylor series of 2^f, 11 terms: 6e-15 of the value.
+// Adding and taking off 1.5 * 2^52 rounds to the integer and leaves it in the
+// low word: no conversions, which take four times an FMA's time.  Logits under
+// 2^-1000 of the maximum, -infinity and NaN have no mass.
+struct Series {            // ln2^i / i!, kept in scalar registers: as operands an FMA takes them in place
+    double c[12];
+    __device__ __forceinline__ Series() {
+        constexpr double k[12] = {1.0, 6.9314718055994531e-01, 2.4022650695910071e-01, 5.5504108664821580e-02,
+                                  9.6181291076284772e-03, 1.3333558146428443e-03, 1.5403530393381608e-04,
+                                  1.5252733804059841e-05, 1.3215486790144309e-06, 1.0178086009239699e-07,
+                                  7.0549116208011234e-09, 4.4455382718708116e-10};
+#pragma unroll
+        for (int i = 0; i < 12; i++) {
+            c[i] = k[i];
+            asm("" : "+s"(c[i]));   // a number like any other to the compiler
+        }
+    }
+    __device__ __forceinline__ double exp2(double f) const {
+        double r = fma(c[11], f, c[10]);
+#pragma unroll
+        for (int i = 9; i >= 0; i--) r = fma(r, f, c[i]);
+        return r;
+    }
+};
+struct Masses {
+    double c, shift;       // y = c x + shift
+    float least;
+    // a maximum of +infinity: only the infinities pass `least`, and y is 0 for them
+    __device__ __forceinline__ Masses(float mx, const VerifyArgs& a) {
+        const bool infinite = mx == INFINITY, none = !(mx > -INFINITY);
+        const double m = infinite || none ? 0.0 : (double)mx;
+        c = infinite ? 0.0 : a.rate;
+        shift = -m * a.rate;
+        least = none ? INFINITY : infinite ? 3.4028234663852886e38f : (float)(m - a.reach);
+    }
+    __device__ __forceinline__ double of(float x, const Series& series) const {
+        constexpr double BIG = 6755399441055744.0;
+        const double y = fma((double)__builtin_amdgcn_fmed3f(x, least, 3.4028234663852886e38f), c, shift);
+        const double t = y + BIG;
+        const double r = series.exp2(y - (t - BIG));
+        const uint64_t u = __builtin_bit_cast(uint64_t, r);
+        const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);   // the integer, modulo 2^32
+        const bool some = x > least;
+        const uint32_t high = some ? (uint32_t)(u >> 32) + (k << 20) : 0, low = some ? (uint32_t)u : 0;
+        return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+    }
+};
 
 __device__ __forceinline__ int draft_count(const VerifyArgs& a, int b) {
     const int n = a.counts ? a.counts[b] : a.drafts;
@@ -91,199 +114,85 @@ __device__ __forceinline__ const float* draft_row(const VerifyArgs& a, int b, in
     return a.draft + ((int64_t)b * a.drafts + i) * a.vocab;
 }
 
-// A thread's logits of a slice (consecutive ones), `pad` past the row's end.
-__device__ __forceinline__ void load_slice(const float* row, int first, int vocab, float pad, float (&x)[PER]) {
-    const int t0 = first + threadIdx.x * PER;
-    if (t0 + PER <= vocab) {
+// A thread's logits of a slice of Q quads per thread; -infinity past the row's end.
+template <int Q>
+__device__ __forceinline__ void load_slice(const float* row, int slice, int vocab, float (&x)[Q][QUAD]) {
+    const int first = slice * Q * (VT * QUAD) + (int)threadIdx.x * QUAD;
+    // no branch around a load: the ones behind it would wait for it
+    if ((slice + 1) * Q * (VT * QUAD) <= vocab) {
 #pragma unroll
-        for (int j = 0; j < PER; j += 4) {   // rows begin at any multiple of 4 bytes
-            const u32x4 w = ld16_a4(reinterpret_cast<const uint8_t*>(row + t0 + j));
-            x[j] = __uint_as_float(w.x); x[j + 1] = __uint_as_float(w.y);
-            x[j + 2] = __uint_as_float(w.z); x[j + 3] = __uint_as_float(w.w);
+        for (int j = 0; j < Q; j++) {   // rows begin at any multiple of 4 bytes
+            const u32x4 w = ld16_a4(reinterpret_cast<const uint8_t*>(row + first + j * (VT * QUAD)));
+            x[j][0] = __uint_as_float(w.x); x[j][1] = __uint_as_float(w.y);
+            x[j][2] = __uint_as_float(w.z); x[j][3] = __uint_as_float(w.w);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < PER; j++) x[j] = t0 + j < vocab ? row[t0 + j] : pad;
+        for (int j = 0; j < Q; j++)
+#pragma unroll
+            for (int i = 0; i < QUAD; i++) {
+                const int t = first + j * (VT * QUAD) + i;
+                const float v = row[t < vocab ? t : vocab - 1];
+                x[j][i] = t < vocab ? v : -INFINITY;
+            }
     }
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
+// Results that another workgroup of the same launch reads: past the XCD's own L2.
+template <typename T>
+__device__ __forceinline__ void store_through(T* p, const T& v) {
+    static_assert(sizeof(T) % 8 == 0, "whole words");
+    uint64_t w[sizeof(T) / 8];
+    __builtin_memcpy(w, &v, sizeof(T));
 #pragma unroll
-    for (int k = 1; k < 64; k *= 2) v += __shfl_xor(v, k);
+    for (int i = 0; i < (int)(sizeof(T) / 8); i++)
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(p) + i, w[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T load_past(const T* p) {
+    uint64_t w[sizeof(T) / 8];
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) / 8); i++)
+        w[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    T v;
+    __builtin_memcpy(&v, w, sizeof(T));
     return v;
 }
-
-template <bool GREEDY>
-__global__ __launch_bounds__(VT) void verify_stats(VerifyArgs a, Work w) {
-    const int slice = blockIdx.x % w.slices, b = blockIdx.x / w.slices, row = blockIdx.y;
-    const int n = draft_count(a, b);
-    const bool of_target = row <= a.drafts;
-    const int i = of_target ? row : row - a.drafts - 1;
-    if (of_target ? i > n : i >= n) return;
-    float x[PER];
-    load_slice(of_target ? target_row(a, b, i) : draft_row(a, b, i), slice * SLICE, a.vocab, -INFINITY, x);
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < PER; j++) m = fmaxf(m, x[j]);   // NaN passes by
-    __shared__ float sm[VT / 64];
-    __shared__ double sz[VT / 64];
-    __shared__ int sa[VT / 64];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    const float wm = wave_max(m);
-    if (lane == 0) sm[wave] = wm;
-    __syncthreads();
-    float mx = sm[0];
-#pragma unroll
-    for (int k = 1; k < VT / 64; k++) mx = fmaxf(mx, sm[k]);
-    double z = 0.0;
-    int arg = -1;
-    if constexpr (GREEDY) {
-        int at = 0x7fffffff;
-#pragma unroll
-        for (int j = PER - 1; j >= 0; j--)
-            if (x[j] == mx) at = slice * SLICE + threadIdx.x * PER + j;
-#pragma unroll
-        for (int k = 1; k < 64; k *= 2) {
-            const int o = __shfl_xor(at, k);
-            at = o < at ? o : at;
-        }
-        if (lane == 0) sa[wave] = at;
-        __syncthreads();
-        arg = sa[0];
-#pragma unroll
-        for (int k = 1; k < VT / 64; k++) arg = sa[k] < arg ? sa[k] : arg;
-    } else {
-        const double c = rate((double)a.temperature);
-        if (mx > -INFINITY)
-#pragma unroll
-            for (int j = 0; j < PER; j++) z += mass(x[j], mx, c);
-        z = wave_sum64(z);
-        if (lane == 0) sz[wave] = z;
-        __syncthreads();
-        z = sz[0];
-#pragma unroll
-        for (int k = 1; k < VT / 64; k++) z += sz[k];
-    }
-    if (threadIdx.x == 0) w.stats[((int64_t)b * w.rows + row) * w.slices + slice] = SliceStats{z, mx, arg};
-}
-
-// A row's maximum and mass from its slices, by 16 lanes (every lane gets them).
-__device__ __forceinline__ void join_slices(const SliceStats* s, int slices, int lane16, double c, float& mx, double& z) {
-    float m = -INFINITY;
-    for (int k = lane16; k < slices; k += 16) m = fmaxf(m, s[k].mx);
-    mx = max16(m);
-    z = 0.0;
-    for (int k = lane16; k < slices; k += 16) {
-        const SliceStats t = s[k];
-        // the slice's mass against the row's maximum
-        if (t.mx > -INFINITY) z += t.z * mass(t.mx, mx, c);
-    }
-#pragma unroll
-    for (int k = 1; k < 16; k *= 2) z += __shfl_xor(z, k);
-}
-// The same for the first maximum.
-__device__ __forceinline__ int join_first(const SliceStats* s, int slices, int lane16) {
-    float m = -INFINITY;
-    for (int k = lane16; k < slices; k += 16) m = fmaxf(m, s[k].mx);
-    m = max16(m);
-    if (m == -INFINITY) return -1;
-    int at = 0x7fffffff;
-    for (int k = lane16; k < slices; k += 16)
-        if (s[k].mx == m && s[k].arg < at) at = s[k].arg;
-#pragma unroll
-    for (int k = 1; k < 16; k *= 2) {
-        const int o = __shfl_xor(at, k);
-        at = o < at ? o : at;
-    }
-    return at;
-}
-
-// How many leading drafts of sequence b stand (the whole workgroup; 16 lanes a draft).
-template <bool GREEDY>
-__device__ int decide(const VerifyArgs& a, const Work& w, int b, int n, int* fail) {
-    const int set = threadIdx.x / 16, lane16 = threadIdx.x & 15;
-    if (threadIdx.x == 0) *fail = n;
-    __syncthreads();
-    const SliceStats* stats = w.stats + (int64_t)b * w.rows * w.slices;
-    const double c = GREEDY ? 0.0 : rate((double)a.temperature);
-    for (int i0 = 0; i0 < n; i0 += VT / 16) {
-        const int i = i0 + set;
-        if (i < n) {
-            const int t = a.draft_tokens[(int64_t)b * a.drafts + i];
-            bool stands = t >= 0 && t < a.vocab;
-            if constexpr (GREEDY) {
-                stands = join_first(stats + (int64_t)i * w.slices, w.slices, lane16) == t && stands;
-            } else {
-                float mp, mq;
-                double zp, zq, q = 1.0;
-                join_slices(stats + (int64_t)i * w.slices, w.slices, lane16, c, mp, zp);
-                if (a.draft) {
-                    join_slices(stats + (int64_t)(a.drafts + 1 + i) * w.slices, w.slices, lane16, c, mq, zq);
-                    q = stands && zq > 0.0 ? mass(draft_row(a, b, i)[t], mq, c) / zq : 0.0;
-                }
-                const double p = stands && zp > 0.0 ? mass(target_row(a, b, i)[t], mp, c) / zp : 0.0;
-                stands = (double)a.uniforms[(int64_t)b * (a.drafts + 1) + i] * q < p && stands;
-            }
-            if (!stands && lane16 == 0) atomicMin(fail, i);
-        }
-        __syncthreads();
-        if (*fail < n) break;   // the same for all: nothing writes it between here and the next barrier
-        __syncthreads();
-    }
-    return *fail;
-}
-
-__device__ __forceinline__ double residual(float x, float y, const Verdict& v, int t, double c, double& p) {
-    p = v.zp > 0.0 ? mass(x, v.mp, c) / v.zp : 0.0;
-    const double q = v.has_q ? mass(y, v.mq, c) / v.zq : t == v.one ? 1.0 : 0.0;
-    return fmax(p - q, 0.0);
-}
-
-__global__ __launch_bounds__(VT) void verify_residual(VerifyArgs a, Work w) {
-    __shared__ int fail;
-    __shared__ Verdict sv;
-    __shared__ double sr[VT / 64], sp[VT / 64];
-    const int slice = blockIdx.x % w.slices, b = blockIdx.x / w.slices;
-    const int n = draft_count(a, b);
-    const int acc = decide<false>(a, w, b, n, &fail);
-    const double c = rate((double)a.temperature);
-    const SliceStats* stats = w.stats + (int64_t)b * w.rows * w.slices;
-    if (threadIdx.x < 16) {
-        Verdict v{0.0, 0.0, 0.f, 0.f, acc, -1, 0, 0};
-        join_slices(stats + (int64_t)acc * w.slices, w.slices, threadIdx.x, c, v.mp, v.zp);
-        if (acc < n) {
-            if (a.draft) {
-                join_slices(stats + (int64_t)(a.drafts + 1 + acc) * w.slices, w.slices, threadIdx.x, c, v.mq, v.zq);
-                v.has_q = v.zq > 0.0;
-            } else {
-                v.one = a.draft_tokens[(int64_t)b * a.drafts + acc];
-            }
-        }
-        if (threadIdx.x == 0) {
-            sv = v;
-            if (slice == 0) w.verdict[b] = v;
-        }
-    }
-    __syncthreads();
-    const Verdict v = sv;
-    float x[PER], y[PER];
-    load_slice(target_row(a, b, acc), slice * SLICE, a.vocab, -INFINITY, x);
-    if (v.has_q) load_slice(draft_row(a, b, acc), slice * SLICE, a.vocab, -INFINITY, y);
-    double r = 0.0, s = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        double p;
-        r += residual(x[j], v.has_q ? y[j] : 0.f, v, slice * SLICE + threadIdx.x * PER + j, c, p);
-        s += p;
-    }
-    r = wave_sum64(r);
-    s = wave_sum64(s);
-    if ((threadIdx.x & 63) == 0) { sr[threadIdx.x / 64] = r; sp[threadIdx.x / 64] = s; }
-    __syncthreads();
+// Whether this workgroup is the last of `of` to get here (thread 0 has stored
+// its result through); the counter is left at zero.
+__device__ __forceinline__ bool last_of(uint32_t* count, uint32_t of) {
+    __shared__ int last;
     if (threadIdx.x == 0) {
-        for (int k = 1; k < VT / 64; k++) { r += sr[k]; s += sp[k]; }
-        w.mass[(int64_t)b * w.slices + slice] = SliceMass{r, s};
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint32_t was = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = was + 1 == of;
+        if (last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    __syncthreads();
+    return last;
+}
+
+// 64-bit values over lanes, without the LDS.
+template <typename F>
+__device__ __forceinline__ double lanes64(F f, double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)f((uint32_t)u) | (uint64_t)f((uint32_t)(u >> 32)) << 32);
+}
+__device__ __forceinline__ double sum16_64(double v) {
+    v += lanes64(lane_xor1, v);
+    v += lanes64(lane_xor2, v);
+    v += lanes64(lane_mirror8, v);
+    return v + lanes64(lane_mirror16, v);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+    v = sum16_64(v);
+    v += lanes64(lane_xor16, v);
+    return v + lanes64(lane_xor32, v);
+}
+__device__ __forceinline__ int wave_min_int(int v) {
+    auto step = [&](uint32_t (*f)(uint32_t)) { const int o = (int)f((uint32_t)v); v = o < v ? o : v; };
+    step(lane_xor1); step(lane_xor2); step(lane_mirror8); step(lane_mirror16); step(lane_xor16); step(lane_xor32);
+    return v;
 }
 
 __device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int acc, int next) {
@@ -293,112 +202,327 @@ __device__ __forceinline__ void write_tokens(const VerifyArgs& a, int b, int acc
     if (threadIdx.x == 0) a.accepted_out[b] = acc;
 }
 
-__global__ __launch_bounds__(VT) void verify_greedy(VerifyArgs a, Work w) {
+// A row's maximum and mass from its slices, by 16 lanes (every lane gets them).
+__device__ __forceinline__ void join_slices(const VerifyArgs& a, const SliceStats* s, int slices, int lane16,
+                                            const Series& series, float& mx, double& z) {
+    mx = -INFINITY;
+    z = 0.0;
+    for (int k = lane16; k < slices; k += 16) {
+        const SliceStats t = s[k];
+        const float m = fmaxf(mx, t.mx);
+        const Masses e(m, a);   // against the larger maximum
+        z = z * e.of(mx, series) + t.z * e.of(t.mx, series);
+        mx = m;
+    }
+    const float m = max16(mx);
+    z = sum16_64(z * Masses(m, a).of(mx, series));
+    mx = m;
+}
+// The first of a row's maxima, from its slices.
+__device__ __forceinline__ int join_first(const SliceStats* s, int slices, int lane16) {
+    float mx = -INFINITY;
+    int at = 0x7fffffff;
+    for (int k = lane16; k < slices; k += 16) {   // ascending: an equal maximum further on is not the first
+        const SliceStats t = s[k];
+        if (t.mx > mx) { mx = t.mx; at = t.arg; }
+    }
+    const float m = max16(mx);
+    if (m == -INFINITY) return -1;
+    at = mx == m ? at : 0x7fffffff;
+#pragma unroll
+    for (int k = 1; k < 16; k *= 2) {
+        const int o = __shfl_xor(at, k);
+        at = o < at ? o : at;
+    }
+    return at;
+}
+
+// The leading drafts of sequence b that stand, and the statistics of the rows
+// behind the first that does not, by the whole workgroup: 16 lanes a draft.  All
+// loads are of known addresses, so they are out at once.
+template <bool GREEDY>
+__device__ __forceinline__ Verdict decide(const VerifyArgs& a, const Work& w, int b) {
     __shared__ int fail;
+    __shared__ Verdict of_set[VT / 16];
+    const int set = threadIdx.x / 16, lane16 = threadIdx.x & 15, n = draft_count(a, b);
+    if (threadIdx.x == 0) fail = n;
+    __syncthreads();
+    const SliceStats* stats = w.stats + (int64_t)b * w.rows * w.slices;
+    const float* picked = w.picked + (int64_t)b * w.rows;
+    const Series series;
+    for (int i0 = 0;; i0 += VT / 16) {
+        const int i = i0 + set;
+        if (i <= n) {
+            const bool drafted = i < a.drafts, with_q = drafted && w.rows > a.drafts + 1;
+            const int t = drafted ? a.draft_tokens[(int64_t)b * a.drafts + i] : -1;
+            const double u = (double)a.uniforms[(int64_t)b * (a.drafts + 1) + i];
+            bool stands = t >= 0 && t < a.vocab;
+            Verdict v{0.0, 0.0, 0.f, 0.f, i, -1, 0, 0};
+            if constexpr (GREEDY) {
+                v.one = join_first(stats + (int64_t)i * w.slices, w.slices, lane16);
+                stands = stands && v.one == t;
+            } else {
+                const float xt = picked[i], yt = with_q ? picked[a.drafts + 1 + i] : 0.f;
+                join_slices(a, stats + (int64_t)i * w.slices, w.slices, lane16, series, v.mp, v.zp);
+                double q = 1.0;
+                if (with_q) {
+                    join_slices(a, stats + (int64_t)(a.drafts + 1 + i) * w.slices, w.slices, lane16, series, v.mq, v.zq);
+                    q = v.zq > 0.0 ? Masses(v.mq, a).of(yt, series) / v.zq : 0.0;
+                }
+                const double p = v.zp > 0.0 ? Masses(v.mp, a).of(xt, series) / v.zp : 0.0;
+                stands = stands && u * q < p;
+                // after the last draft the next token is the target's alone
+                v.has_q = with_q && i < n && v.zq > 0.0;
+                if (!a.draft && i < n) v.one = t;
+            }
+            if (lane16 == 0) {
+                of_set[set] = v;
+                if (!stands) atomicMin(&fail, i);
+            }
+        }
+        __syncthreads();
+        const int acc = fail;   // the same for all threads: the next write waits for the barrier
+        const Verdict v = of_set[acc < i0 + VT / 16 ? acc - i0 : 0];
+        __syncthreads();
+        if (acc < i0 + VT / 16) return v;
+    }
+}
+
+template <bool GREEDY, int Q>
+__global__ __launch_bounds__(VT) void verify_stats(VerifyArgs a, Work w) {
+    const int slice = blockIdx.x % w.slices, b = blockIdx.x / w.slices, row = blockIdx.y;
+    const int n = draft_count(a, b);
+    const bool of_target = row <= a.drafts;
+    const int i = of_target ? row : row - a.drafts - 1;
+    if (of_target ? i > n : i >= n) return;
+    const float* logits = of_target ? target_row(a, b, i) : draft_row(a, b, i);
+    float x[Q][QUAD];
+    load_slice<Q>(logits, slice, a.vocab, x);
+    if (threadIdx.x == 0 && i < a.drafts) {
+        const int t = a.draft_tokens[(int64_t)b * a.drafts + i];
+        if (t >= 0 && t < a.vocab && t / (Q * VT * QUAD) == slice) w.picked[(int64_t)b * w.rows + row] = logits[t];
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < Q; j++)
+#pragma unroll
+        for (int k = 0; k < QUAD; k++) m = fmaxf(m, x[j][k]);   // NaN passes by
+    __shared__ float sm[WAVES];
+    __shared__ double sz[WAVES];
+    __shared__ int sa[WAVES];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    m = wave_max(m);
+    if (lane == 0) sm[wave] = m;
+    __syncthreads();
+    float mx = sm[0];
+#pragma unroll
+    for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, sm[k]);
+    double z = 0.0;
+    int arg = -1;
+    if constexpr (GREEDY) {
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int j = Q - 1; j >= 0; j--)
+#pragma unroll
+            for (int k = QUAD - 1; k >= 0; k--)
+                if (x[j][k] == mx) at = (slice * Q + j) * (VT * QUAD) + (int)threadIdx.x * QUAD + k;
+        at = wave_min_int(at);
+        if (lane == 0) sa[wave] = at;
+        __syncthreads();
+        arg = sa[0];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) arg = sa[k] < arg ? sa[k] : arg;
+    } else {
+        const Masses e(mx, a);
+        const Series series;
+#pragma unroll
+        for (int j = 0; j < Q; j++)
+#pragma unroll
+            for (int k = 0; k < QUAD; k++) z += e.of(x[j][k], series);
+        z = wave_sum64(z);
+        if (lane == 0) sz[wave] = z;
+        __syncthreads();
+        z = sz[0];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) z += sz[k];
+    }
+    if (threadIdx.x == 0) w.stats[((int64_t)b * w.rows + row) * w.slices + slice] = SliceStats{z, mx, arg};
+}
+
+__global__ __launch_bounds__(VT) void verify_greedy(VerifyArgs a, Work w) {
     const int b = blockIdx.x;
-    const int acc = decide<true>(a, w, b, draft_count(a, b), &fail);
-    const int next = join_first(w.stats + ((int64_t)b * w.rows + acc) * w.slices, w.slices, threadIdx.x & 15);
-    write_tokens(a, b, acc, next);
+    const Verdict v = decide<true>(a, w, b);
+    write_tokens(a, b, v.accepted, v.one);
 }
 
-// Inclusive sums over the workgroup's threads, in thread order.
-__device__ __forceinline__ double block_scan(double v, double* sh) {
+// max(p - q, 0) of a token, and p.
+struct Residual {
+    Series series;
+    Masses p, q;
+    double ip, iq;         // 1 / masses, 0 without any
+    int one;
+    __device__ __forceinline__ Residual(const Verdict& v, const VerifyArgs& a)
+        : p(v.mp, a), q(v.mq, a), ip(v.zp > 0.0 ? 1.0 / v.zp : 0.0), iq(v.has_q ? 1.0 / v.zq : 0.0), one(v.one) {}
+    __device__ __forceinline__ double of(float x, float y, int t, double& pt) const {
+        pt = p.of(x, series) * ip;
+        return fmax(pt - (iq > 0.0 ? q.of(y, series) * iq : t == one ? 1.0 : 0.0), 0.0);
+    }
+};
+
+// Inclusive sums over the wavefront's lanes: within rows of 16, then rows 0 and 2
+// into 1 and 3, then the lower half into the upper.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double v) {   // 0 where the lane or its row takes no part
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan64(double v) {
+    v += dpp64<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+    v += dpp64<0x112, 0xF>(v);
+    v += dpp64<0x114, 0xF>(v);
+    v += dpp64<0x118, 0xF>(v);
+    v += dpp64<0x142, 0xA>(v);   // row_bcast 15
+    return v + dpp64<0x143, 0xC>(v);   // row_bcast 31
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+template <int Q>
+__global__ __launch_bounds__(VT) void verify_draw(VerifyArgs a, Work w) {
+    __shared__ double sr[WAVES], sp[WAVES], part[Q][WAVES];
+    __shared__ int next;
+    const int slice = blockIdx.x % w.slices, b = blockIdx.x / w.slices;
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const double o = __shfl_up(v, k);
-        if (lane >= k) v += o;
-    }
-    __syncthreads();
-    if (lane == 63) sh[wave] = v;
-    __syncthreads();
-    for (int k = 0; k < wave; k++) v += sh[k];
-    return v;
-}
-
-__global__ __launch_bounds__(VT) void verify_select(VerifyArgs a, Work w) {
-    __shared__ double sh[VT / 64], before_at;
-    __shared__ int first, last;
-    const int b = blockIdx.x, tid = threadIdx.x;
-    Verdict v = w.verdict[b];
-    const SliceMass* m = w.mass + (int64_t)b * w.slices;
+    Verdict v = decide<false>(a, w, b);
     const double u = (double)a.uniforms[(int64_t)b * (a.drafts + 1) + a.drafts];
-    const double c = rate((double)a.temperature);
-    // runs of slices per thread
-    const int per = (w.slices + VT - 1) / VT, k0 = tid * per < w.slices ? tid * per : w.slices,
-              k1 = k0 + per < w.slices ? k0 + per : w.slices;
-    bool of_p = false;
-    double mine = 0.0, upto = 0.0, total = 0.0;
-    for (int pass = 0; pass < 2; pass++) {
-        of_p = pass == 1;
-        mine = 0.0;
-        for (int k = k0; k < k1; k++) mine += of_p ? m[k].p : m[k].r;
-        upto = block_scan(mine, sh);
-        if (tid == VT - 1) before_at = upto;
-        __syncthreads();
-        total = before_at;
-        if (total > 0.0) break;   // the same for all
-        __syncthreads();
-    }
-    int next = -1;
-    if (total > 0.0) {
-        if (of_p) { v.has_q = 0; v.one = -1; }
-        const double want = u * total;
-        if (tid == 0) { first = w.slices; last = -1; }
-        __syncthreads();
-        double cum = upto - mine;
-        int found = w.slices, some = -1;
-        for (int k = k0; k < k1; k++) {
-            const double s = of_p ? m[k].p : m[k].r;
-            cum += s;
-            if (s > 0.0) {
-                some = k;
-                if (cum > want && found == w.slices) found = k;
-            }
-        }
-        if (found < w.slices) atomicMin(&first, found);
-        if (some >= 0) atomicMax(&last, some);
-        __syncthreads();
-        const int slice = first < w.slices ? first : last;   // a draw past the last border by rounding
-        __syncthreads();
-        if (slice >= k0 && slice < k1) {
-            double s = upto - mine;
-            for (int k = k0; k < slice; k++) s += of_p ? m[k].p : m[k].r;
-            before_at = s;
-        }
-        if (tid == 0) { first = 0x7fffffff; last = -1; }
-        __syncthreads();
-        float x[PER], y[PER];
-        load_slice(target_row(a, b, v.accepted), slice * SLICE, a.vocab, -INFINITY, x);
-        if (v.has_q) load_slice(draft_row(a, b, v.accepted), slice * SLICE, a.vocab, -INFINITY, y);
-        double r[PER], sum = 0.0;
-        const int t0 = slice * SLICE + tid * PER;
+    const float* target = target_row(a, b, v.accepted);
+    const float* draft = v.has_q ? draft_row(a, b, v.accepted) : target;
+    const Residual e(v, a);
+    float x[Q][QUAD], y[Q][QUAD];
+    auto token = [&](int s, int j, int k) { return (s * Q + j) * (VT * QUAD) + (int)threadIdx.x * QUAD + k; };
+    load_slice<Q>(target, slice, a.vocab, x);
+    load_slice<Q>(draft, slice, a.vocab, y);
+    double r = 0.0, s = 0.0;
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
+    for (int j = 0; j < Q; j++)
+#pragma unroll
+        for (int k = 0; k < QUAD; k++) {
             double p;
-            r[j] = residual(x[j], v.has_q ? y[j] : 0.f, v, t0 + j, c, p);
-            sum += r[j];
+            r += e.of(x[j][k], y[j][k], token(slice, j, k), p);
+            s += p;
         }
-        cum = before_at + (block_scan(sum, sh) - sum);
-        int at = 0x7fffffff, most = -1;
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            cum += r[j];
-            if (r[j] > 0.0) {
-                most = t0 + j;
-                if (cum > want && at == 0x7fffffff) at = t0 + j;
-            }
-        }
-        if (at != 0x7fffffff) atomicMin(&first, at);
-        if (most >= 0) atomicMax(&last, most);
-        __syncthreads();
-        next = first != 0x7fffffff ? first : last;
+    r = wave_sum64(r);
+    s = wave_sum64(s);
+    if (lane == 0) { sr[wave] = r; sp[wave] = s; }
+    __syncthreads();
+    SliceMass* m = w.mass + (int64_t)b * w.slices;
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < WAVES; k++) { r += sr[k]; s += sp[k]; }
+        store_through(m + slice, SliceMass{r, s});
     }
+    if (!last_of(w.drawn + b * COUNTER_STRIDE, (uint32_t)w.slices)) return;
+
+    // every wavefront adds the slices up for itself, a lane a slice
+    auto slice_of = [&](int k0) {
+        return k0 + lane < w.slices ? load_past(m + k0 + lane) : SliceMass{0.0, 0.0};
+    };
+    double total = 0.0, total_p = 0.0;
+    SliceMass mine{0.0, 0.0};
+    for (int k0 = 0; k0 < w.slices; k0 += 64) {
+        mine = slice_of(k0);
+        total += wave_sum64(mine.r);
+        total_p += wave_sum64(mine.p);
+    }
+    const bool of_p = !(total > 0.0);   // nothing left over: the target's own distribution
+    if (of_p) {
+        total = total_p;
+        v.has_q = 0;
+        v.one = -1;
+    }
+    if (!(total > 0.0)) {
+        write_tokens(a, b, v.accepted, -1);
+        return;
+    }
+    const double want = u * total;
+    // the piece (of those that the lanes hold, `cum` before them) that holds the
+    // draw, else the last with any mass: a draw past the last border by rounding
+    double cum = 0.0, before = 0.0;
+    int at = -1;
+    auto search = [&](double x1, int k0) {
+        const double upto = cum + wave_scan64(x1);
+        const uint64_t over = __ballot(x1 > 0.0 && upto > want), any = __ballot(x1 > 0.0);
+        if (any) {
+            const int k = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)any);
+            at = k0 + k;
+            before = lane64(upto - x1, __builtin_amdgcn_readfirstlane(k));
+        }
+        cum = lane64(upto, 63);
+        return over != 0;
+    };
+    for (int k0 = 0; k0 < w.slices; k0 += 64) {
+        if (w.slices > 64) mine = slice_of(k0);
+        if (search(of_p ? mine.p : mine.r, k0)) break;
+    }
+    const int chosen = at;
+    const Residual e2(v, a);
+    load_slice<Q>(target, chosen, a.vocab, x);
+    load_slice<Q>(draft, chosen, a.vocab, y);
+    // sums of the slice's pieces: a quad of each of a wavefront's lanes
+#pragma unroll
+    for (int j = 0; j < Q; j++) {
+        double sum = 0.0, p;
+#pragma unroll
+        for (int k = 0; k < QUAD; k++) sum += e2.of(x[j][k], y[j][k], token(chosen, j, k), p);
+        sum = wave_sum64(sum);
+        if (lane == 0) part[j][wave] = sum;
+    }
+    if (threadIdx.x == 0) next = -1;
+    __syncthreads();
+    cum = before;
+    search(lane < Q * WAVES ? part[lane / WAVES][lane % WAVES] : 0.0, 0);
+    if (at % WAVES == wave) {   // one wavefront looks through the piece
+        const int piece = at / WAVES, t0 = token(chosen, piece, 0);
+        double r1[QUAD], sum = 0.0, p;
+#pragma unroll
+        for (int k = 0; k < QUAD; k++) {
+            float xk = x[0][k], yk = y[0][k];
+#pragma unroll
+            for (int j = 1; j < Q; j++) { xk = piece == j ? x[j][k] : xk; yk = piece == j ? y[j][k] : yk; }
+            r1[k] = e2.of(xk, yk, t0 + k, p);
+            sum += r1[k];
+        }
+        cum = before;
+        search(sum, 0);
+        if (lane == at) {
+            int found = -1;
+            bool over = false;
+#pragma unroll
+            for (int k = 0; k < QUAD; k++) {
+                before += r1[k];
+                if (r1[k] > 0.0 && !over) {
+                    found = t0 + k;
+                    over = before > want;
+                }
+            }
+            next = found;
+        }
+    }
+    __syncthreads();
     write_tokens(a, b, v.accepted, next);
 }
 
+// Logits of a slice: small ones where there are few slices to a row anyway.
+int quads_of(int vocab) { return vocab <= 32768 ? 1 : 4; }
+
 size_t layout(int batch, int drafts, int vocab, bool draft, uint8_t* base, Work* w) {
-    w->slices = (vocab + SLICE - 1) / SLICE;
+    const int slice = VT * QUAD * quads_of(vocab);
+    w->slices = (vocab + slice - 1) / slice;
     w->rows = drafts + 1 + (draft ? drafts : 0);
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -406,10 +530,24 @@ size_t layout(int batch, int drafts, int vocab, bool draft, uint8_t* base, Work*
         at += (n + 15) & ~(size_t)15;
         return p;
     };
-    w->stats = reinterpret_cast<SliceStats*>(take(sizeof(SliceStats) * (size_t)batch * w->rows * w->slices));
-    w->verdict = reinterpret_cast<Verdict*>(take(sizeof(Verdict) * (size_t)batch));
+    // the counters come first in every workspace: what a call leaves there is zero for any other
+    w->drawn = reinterpret_cast<uint32_t*>(take((size_t)4 * VERIFY_BATCH * COUNTER_STRIDE));
+    w->picked = reinterpret_cast<float*>(take(sizeof(float) * (size_t)batch * w->rows));
     w->mass = reinterpret_cast<SliceMass*>(take(sizeof(SliceMass) * (size_t)batch * w->slices));
+    w->stats = reinterpret_cast<SliceStats*>(take(sizeof(SliceStats) * (size_t)batch * w->rows * w->slices));
     return at;
+}
+
+template <int Q>
+void launch_sized(const VerifyArgs& a, const Work& w, hipStream_t s) {
+    const dim3 slices((uint32_t)w.slices * a.batch), rows(slices.x, w.rows);
+    if (a.temperature <= 0.f) {
+        verify_stats<true, Q><<<rows, VT, 0, s>>>(a, w);
+        verify_greedy<<<dim3(a.batch), VT, 0, s>>>(a, w);
+    } else {
+        verify_stats<false, Q><<<rows, VT, 0, s>>>(a, w);
+        verify_draw<Q><<<slices, VT, 0, s>>>(a, w);
+    }
 }
 
 }  // namespace
@@ -419,19 +557,13 @@ size_t verify_workspace(int batch, int drafts, int vocab) {
     return layout(batch, drafts, vocab, true, nullptr, &w);
 }
 
-hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
+hipError_t launch_verify(VerifyArgs a, hipStream_t s) {
     Work w;
-    const bool greedy = a.temperature <= 0.f;
-    layout(a.batch, a.drafts, a.vocab, a.draft && !greedy, a.work, &w);
-    const dim3 grid((uint32_t)w.slices * a.batch, w.rows);
-    if (greedy) {
-        verify_stats<true><<<grid, VT, 0, s>>>(a, w);
-        verify_greedy<<<dim3(a.batch), VT, 0, s>>>(a, w);
-    } else {
-        verify_stats<false><<<grid, VT, 0, s>>>(a, w);
-        verify_residual<<<dim3((uint32_t)w.slices * a.batch), VT, 0, s>>>(a, w);
-        verify_select<<<dim3(a.batch), VT, 0, s>>>(a, w);
-    }
+    a.rate = a.temperature > 0.f ? 1.4426950408889634074 / (double)a.temperature : 0.0;
+    a.reach = a.temperature > 0.f ? 1000.0 / a.rate : 0.0;
+    layout(a.batch, a.drafts, a.vocab, a.draft && a.temperature > 0.f, a.work, &w);
+    if (quads_of(a.vocab) == 1) launch_sized<1>(a, w, s);
+    else launch_sized<4>(a, w, s);
     return hipGetLastError();
 }
 
