@@ -125,18 +125,12 @@ struct Tile {
     float m, l;            // reference and (the lane's part of the) sum
     f4 o[2 * NB];          // dims 16 t + 4 g .. + 3 of row `lane & 15`
 
-    // q: the row's head_dim floats (null: an empty row)
-    __device__ __forceinline__ void init(const float* q, int g, float scale) {
+    __device__ __forceinline__ void init(const f4 (&q)[2 * NB], float scale) {
         float x[NB][8], top = 0.f;
 #pragma unroll
         for (int i = 0; i < NB; i++) {
-            f4 a{0.f, 0.f, 0.f, 0.f}, b{0.f, 0.f, 0.f, 0.f};
-            if (q) {
-                a = *reinterpret_cast<const f4*>(q + 32 * i + 8 * g);
-                b = *reinterpret_cast<const f4*>(q + 32 * i + 8 * g + 4);
-            }
 #pragma unroll
-            for (int j = 0; j < 4; j++) { x[i][j] = a[j]; x[i][4 + j] = b[j]; }
+            for (int j = 0; j < 4; j++) { x[i][j] = q[2 * i][j]; x[i][4 + j] = q[2 * i + 1][j]; }
 #pragma unroll
             for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[i][j]));
         }
@@ -158,23 +152,6 @@ struct Tile {
         for (int t = 0; t < 2 * NB; t++) o[t] = f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    // Scores (times log2 e) plus exponents of a record's 32 positions: s[4 t + r] is position 16 t + 4 g + r.
-    template <bool KQ4>
-    __device__ __forceinline__ void scores(const h8 (&kf)[2][NB], const Record<KQ4, NB>& k, const h8& e, float (&s)[8]) const {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            f4 sum{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                f4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], ql[i], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], qh[i], c, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; r++) sum[r] = fmaf(c[r], (float)k.d[i][4 * t + r], sum[r]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[4 * t + r] = fmaf(sum[r], qinv, (float)e[4 * t + r]);
-        }
-    }
     __device__ __forceinline__ void mask(float (&s)[8], int first, int g) const {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -207,6 +184,37 @@ struct Tile {
         split8(p, ph, pl);
     }
 };
+
+// Scores (times log2 e) plus exponents of a record's 32 positions for R tiles:
+// s[x][4 t + r] is position 16 t + 4 g + r.  All of a half's products go out
+// before the first result is needed: one MFMA's result takes several others' time.
+template <int NB, int R>
+__device__ __forceinline__ void scores(const Tile<NB> (&t)[R], const h8 (&kf)[2][NB], const h8 (&dk)[NB], const h8& e,
+                                       float (&s)[R][8]) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            f4 sum{0.f, 0.f, 0.f, 0.f};
+            constexpr int TOGETHER = 2;
+#pragma unroll
+            for (int i0 = 0; i0 < NB; i0 += TOGETHER) {
+                f4 c[TOGETHER];
+#pragma unroll
+                for (int i = 0; i < TOGETHER && i0 + i < NB; i++)
+                    c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i0 + i], t[x].ql[i0 + i], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < TOGETHER && i0 + i < NB; i++)
+                    c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][i0 + i], t[x].qh[i0 + i], c[i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < TOGETHER && i0 + i < NB; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sum[r] = fmaf(c[i][r], (float)dk[i0 + i][4 * h + r], sum[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[x][4 * h + r] = fmaf(sum[r], t[x].qinv, (float)e[4 * h + r]);
+        }
+}
 
 // Work of one launch.  An entry is a tile of query rows with the records it
 // sees; its records are cut into chunks, one workgroup each.
@@ -251,6 +259,20 @@ __device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
     v += lane_xor16(v);
     return v + lane_xor32(v);
 }
+// Inclusive sums over the lanes: within rows of 16, then rows 0 and 2 into 1 and
+// 3, then the lower half into the upper.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ int wave_scan_int(int v) {
+    v += dpp_or_zero<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112, 0xF>(v);
+    v += dpp_or_zero<0x114, 0xF>(v);
+    v += dpp_or_zero<0x118, 0xF>(v);
+    v += dpp_or_zero<0x142, 0xA>(v);   // row_bcast 15
+    return v + dpp_or_zero<0x143, 0xC>(v);   // row_bcast 31
+}
 // The cut that holds `item`, or (by_entry) the one of entry `item`; entry -1: an
 // item that no entry needs.  Every wavefront works it out from the lengths in
 // memory: one ratio of chunks to records for the whole batch, as high as the
@@ -290,12 +312,7 @@ __device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int
         const int e = e0 + lane;
         if (pl.entries > 64) look(e);
         const int n = chunks(ratio, r.y - r.x);
-        int upto = n;
-#pragma unroll
-        for (int k = 1; k < 64; k *= 2) {
-            const int v = __shfl_up(upto, k);
-            if (lane >= k) upto += v;
-        }
+        const int upto = wave_scan_int(n);
         const bool mine = by_entry ? e == item : item >= before + upto - n && item < before + upto;
         const uint64_t who = __ballot(mine);
         if (who) {
@@ -329,17 +346,66 @@ __device__ __forceinline__ void join_weights(float& m, float mk, float& f, float
     m = mn;
 }
 
-// One workgroup: WR x WK wavefronts, each 16 R query rows of a kv head over every
-// WK-th record of the chunk.  Bound by instruction issue where many rows share
-// the records (prompts), by the loads' latency where few do.  FUSE: the
-// workgroup that finishes an entry's last chunk joins them.
-template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, bool PRE, bool FUSE>
+// Takes the 16 query rows from `first_row` on of a kv head (own rows: of sequence
+// b; a prefix's: of all sequences) for a tile: asks for the lane's part of them,
+// narrows the range of positions that all of them see, and returns where the
+// lane's row goes in `out` (-1: none).
+template <int NB, bool PRE>
+__device__ __forceinline__ int64_t load_rows(const KvAttnArgs& a, Tile<NB>& t, f4 (&q)[2 * NB], int first_row, int b,
+                                             int head, const KvSpan& sp, int& edge_last, int& edge_before) {
+    const int lane = threadIdx.x & 63, tokens = a.rows.tokens, group = (int)a.by_group.d;
+    const int row = first_row + (lane & 15);
+    int i, bb = b, token;
+    KvSpan s = sp;
+    bool there;
+    if constexpr (PRE) {
+        token = a.by_group.div(row);
+        bb = a.by_tokens.div(token);
+        i = a.by_tokens.mod(token, bb);
+        there = bb < a.rows.batch;
+        if (there) s = kv_span(a.rows, a.cache, bb);
+    } else {
+        token = i = a.by_group.div(row);
+        there = i < tokens;
+    }
+    there = there && i >= s.lo && i < s.hi;
+    const int64_t at = (int64_t)bb * tokens + i;
+    const int h = head * group + a.by_group.mod(row, token);
+    // rows that are not there read the call's first (kv head `head` of it) and count as zeros
+    const float* src = a.q + (there ? at * a.q_stride + h * (NB * 32) : (int64_t)head * group * (NB * 32)) + 8 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        q[2 * i] = *reinterpret_cast<const f4*>(src + 32 * i);
+        q[2 * i + 1] = *reinterpret_cast<const f4*>(src + 32 * i + 4);
+    }
+    // positions in the cache at hand; an empty row sees all of the chunk
+    const int pos = s.start + i;
+    t.last = !there ? 0x7fffffff : PRE ? a.prefix_len - 1 : pos;
+    t.before = !there || a.window <= 0 ? -1 : (PRE ? a.prefix_len : 0) + pos - a.window;
+    int el = t.last, eb = t.before;
+#pragma unroll
+    for (int k = 1; k < 16; k *= 2) {
+        const int ol = __shfl_xor(el, k), ob = __shfl_xor(eb, k);
+        el = el < ol ? el : ol;
+        eb = eb > ob ? eb : ob;
+    }
+    el = __builtin_amdgcn_readfirstlane(el);
+    eb = __builtin_amdgcn_readfirstlane(eb);
+    edge_last = el < edge_last ? el : edge_last;
+    edge_before = eb > edge_before ? eb : edge_before;
+    return there ? at * a.out_stride + h * (NB * 32) : -1;
+}
+
+// One workgroup: 16 R query rows of a kv head over a chunk of records, every
+// fourth of them to a wavefront.  Bound by instruction issue (about 200 vector
+// instructions a record and tile at head_dim 64, 300 at 128), by the loads'
+// latency where a wavefront has a record or two.  FUSE: the workgroup that
+// finishes an entry's last chunk joins them.
+template <int NB, bool KQ4, bool VQ4, int R, bool PRE, bool FUSE>
 __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl, int wg, float* lds) {
-    static_assert(WR * WK == WAVES, "four wavefronts to a tile");
-    constexpr int HD = NB * 32, ROWS = 16 * R * WR;
+    constexpr int HD = NB * 32, ROWS = 16 * R;
     const int kvh = a.cache.kv_heads, item = a.by_kv_heads.div(wg), head = wg - item * kvh, group = (int)a.by_group.d;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x & 63, g = lane >> 4;
-    const int wr = wave % WR, wk = wave / WR % WK;
 
     // which rows and records
     int b = 0, tile, r0, r1, entry = 0, chunks = 1, first_item = 0, at_item = item;   // at_item: place in the workspace
@@ -353,15 +419,9 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         r1 = low + (int)((int64_t)n * (k + 1) / per);
     } else {
         if (pl.whole) {
-            // the longest tiles first; with keys to a wavefront (WK = 1), the long
-            // tile's four wavefronts share the SIMDs with a short one's
             const int k = pl.by_batch.div(item);
             b = pl.by_batch.mod(item, k);
-            tile = pl.tiles - 1 - k;
-            if (WK == 1 && wave >= WAVES) {
-                if (k == tile) return;
-                tile = k;
-            }
+            tile = pl.tiles - 1 - k;   // the longest first
             at_item = b * pl.tiles + tile;
             sp = kv_span(a.rows, a.cache, b);
             const int2 r = own_records(a, pl, sp, tile);
@@ -389,65 +449,46 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
     constexpr int64_t KREC = kv_record_bytes(KQ4, NB, false), VREC = kv_record_bytes(VQ4, NB, true);
     Record<KQ4, NB> k;
     VRecord<VQ4, NB> v;
-    int rec = r0 + wk;
-    if (rec < r1) {
-        k.load(kb + rec * KREC, lane);
-        v.load(vb + rec * VREC, lane);
-    }
-
-    // the wavefront's query rows
+    int rec = r0 + wave;
+    auto load_record = [&] {
+        if (rec < r1) {
+            k.load(kb + rec * KREC, lane);
+            v.load(vb + rec * VREC, lane);
+        }
+    };
+    // A prefix's rows are known only once their sequences' lengths are there: its
+    // record goes first.  Loads come back in order, so an own chunk asks for its
+    // queries, which are needed first, before its record.
+    if constexpr (PRE) load_record();
     Tile<NB> t[R];
     int64_t out_at[R];     // element of `out` (-1: not a row)
     int edge_last = 0x7fffffff, edge_before = -1;   // records inside need no mask
     const int tokens = a.rows.tokens;
+    {
+        f4 q[R][2 * NB];
 #pragma unroll
-    for (int x = 0; x < R; x++) {
-        const int row = tile * ROWS + (wr * R + x) * 16 + (lane & 15);
-        int i, bb = b;
-        KvSpan s = sp;
-        bool there;
-        if constexpr (PRE) {
-            const int token = a.by_group.div(row);
-            bb = a.by_tokens.div(token);
-            i = a.by_tokens.mod(token, bb);
-            there = bb < a.rows.batch;
-            if (there) s = kv_span(a.rows, a.cache, bb);
-        } else {
-            i = a.by_group.div(row);
-            there = i < tokens;
-        }
-        there = there && i >= s.lo && i < s.hi;
-        const int64_t at = (int64_t)bb * tokens + i;
-        const int h = head * group + (PRE ? a.by_group.mod(row, bb * tokens + i) : a.by_group.mod(row, i));
-        out_at[x] = there ? at * a.out_stride + h * HD : -1;
-        t[x].init(there ? a.q + at * a.q_stride + h * HD : nullptr, g, a.scale);
-        // positions in the cache at hand; an empty row sees all of the chunk
-        const int pos = s.start + i;
-        t[x].last = !there ? 0x7fffffff : PRE ? a.prefix_len - 1 : pos;
-        t[x].before = !there || a.window <= 0 ? -1 : (PRE ? a.prefix_len : 0) + pos - a.window;
-        int el = t[x].last, eb = t[x].before;
+        for (int x = 0; x < R; x++)
+            out_at[x] = load_rows<NB, PRE>(a, t[x], q[x], tile * ROWS + x * 16, b, head, sp, edge_last, edge_before);
+        if constexpr (!PRE) load_record();
 #pragma unroll
-        for (int k = 1; k < 16; k *= 2) {
-            const int ol = __shfl_xor(el, k), ob = __shfl_xor(eb, k);
-            el = el < ol ? el : ol;
-            eb = eb > ob ? eb : ob;
+        for (int x = 0; x < R; x++) {
+            if (out_at[x] < 0) {
+#pragma unroll
+                for (int i = 0; i < 2 * NB; i++) q[x][i] = f4{0.f, 0.f, 0.f, 0.f};
+            }
+            t[x].init(q[x], a.scale);
         }
-        el = __builtin_amdgcn_readfirstlane(el);
-        eb = __builtin_amdgcn_readfirstlane(eb);
-        edge_last = el < edge_last ? el : edge_last;
-        edge_before = eb > edge_before ? eb : edge_before;
     }
     if (PRE && edge_last > a.prefix_len - 1) edge_last = a.prefix_len - 1;
 
-    for (; rec < r1; rec += WK) {
-        const int next = rec + WK < r1 ? rec + WK : rec;
+    for (; rec < r1; rec += WAVES) {
+        const int next = rec + WAVES < r1 ? rec + WAVES : rec;
         float s[R][8];
         {
             h8 kf[2][NB];
 #pragma unroll
             for (int i = 0; i < NB; i++) { kf[0][i] = k.q[i].k(0); kf[1][i] = k.q[i].k(1); }
-#pragma unroll
-            for (int x = 0; x < R; x++) t[x].scores(kf, k, v.e, s[x]);
+            scores<NB, R>(t, kf, k.d, v.e, s);
         }
         k.load(kb + next * KREC, lane);
         if (rec * KV_GROUP + KV_GROUP - 1 > edge_last || rec * KV_GROUP <= edge_before) {
@@ -480,7 +521,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
     }
 
     const bool direct = pl.whole == 1 || (FUSE && chunks == 1);
-    if constexpr (WK > 1) {
+    {
         // the wavefronts' records meet in LDS, each wavefront summing a share of the dims in order
         auto so = reinterpret_cast<float (*)[16 * R][HD + 4]>(lds);
         auto sm = reinterpret_cast<float (*)[16 * R][2]>(lds + WAVES * 16 * R * (HD + 4));
@@ -495,23 +536,22 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
 #pragma unroll
         for (int x = 0; x < R; x++) {
             const int row = x * 16 + (lane & 15);
-            float mx = -INFINITY, sum = 0.f, f[WK];
+            float mx = -INFINITY, sum = 0.f, f[WAVES];
 #pragma unroll
-            for (int w = 0; w < WK; w++) mx = fmaxf(mx, sm[wr + w * WR][row][0]);
+            for (int w = 0; w < WAVES; w++) mx = fmaxf(mx, sm[w][row][0]);
 #pragma unroll
-            for (int w = 0; w < WK; w++) {
-                const float mw = sm[wr + w * WR][row][0];
+            for (int w = 0; w < WAVES; w++) {
+                const float mw = sm[w][row][0];
                 f[w] = mw == mx ? 1.f : __builtin_amdgcn_exp2f(mw - mx);
-                sum = fmaf(f[w], sm[wr + w * WR][row][1], sum);
+                sum = fmaf(f[w], sm[w][row][1], sum);
             }
-            const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + wr * R * 16 + row;
+            const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + row;
             const float inv = 1.f / sum;
             if (out_at[x] < 0) continue;
-            for (int d = wk; d < 2 * NB; d += WK) {
+            for (int d = wave; d < 2 * NB; d += WAVES) {
                 f4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < WK; w++)
-                    acc += f[w] * *reinterpret_cast<const f4*>(&so[wr + w * WR][row][16 * d + 4 * g]);
+                for (int w = 0; w < WAVES; w++) acc += f[w] * *reinterpret_cast<const f4*>(&so[w][row][16 * d + 4 * g]);
                 float* o = pl.o + part * HD + 16 * d + 4 * g;
                 if (direct) {
                     *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = acc * inv;
@@ -522,26 +562,9 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
                     *reinterpret_cast<f4*>(o) = acc;
                 }
             }
-            if (!direct && wk == 0 && g == 0) {
+            if (!direct && wave == 0 && g == 0) {
                 if constexpr (FUSE) store_through(pl.ml + part * 2, f2{mx, sum});
                 else *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{mx, sum};
-            }
-        }
-    } else {
-#pragma unroll
-        for (int x = 0; x < R; x++) {
-            if (out_at[x] < 0) continue;
-            if (direct) {
-                const float inv = 1.f / t[x].l;
-#pragma unroll
-                for (int d = 0; d < 2 * NB; d++)
-                    *reinterpret_cast<f4*>(a.out + out_at[x] + 16 * d + 4 * g) = t[x].o[d] * inv;
-            } else {
-                const int trow = (wr * R + x) * 16 + (lane & 15);
-                const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + trow;
-#pragma unroll
-                for (int d = 0; d < 2 * NB; d++) *reinterpret_cast<f4*>(pl.o + part * HD + 16 * d + 4 * g) = t[x].o[d];
-                if (g == 0) *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{t[x].m, t[x].l};
             }
         }
     }
@@ -619,18 +642,16 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
 }
 
 // The call's own chunks, and (RP) the prefix's before them, 16 RP rows to a wavefront.
-template <int NB, bool KQ4, bool VQ4, int R, int WR, int WK, int RP>
-__global__ __launch_bounds__(WK == 1 ? 2 * THREADS : THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(
-    KvAttnArgs a, Plan own, Plan pre) {
-    constexpr int MOST = RP > (WK > 1 ? R : 0) ? RP : WK > 1 ? R : 0;   // tiles of a wavefront that meet in LDS
-    __shared__ __align__(16) float lds[MOST > 0 ? WAVES * 16 * MOST * (NB * 32 + 6) + 4 : 4];
-    static_assert(RP == 0 || WK > 1, "the prefix's chunks take four wavefronts");
+template <int NB, bool KQ4, bool VQ4, int R, int RP>
+__global__ __launch_bounds__(THREADS, NB == 8 ? 1 : 2) void kv_attention_kernel(KvAttnArgs a, Plan own, Plan pre) {
+    constexpr int MOST = RP > R ? RP : R;
+    __shared__ __align__(16) float lds[WAVES * 16 * MOST * (NB * 32 + 6) + 4];
     if constexpr (RP > 0) {
         const int before = pre.items * a.cache.kv_heads;
-        if ((int)blockIdx.x < before) attend_chunk<NB, KQ4, VQ4, RP, 1, 4, true, false>(a, pre, blockIdx.x, lds);
-        else attend_chunk<NB, KQ4, VQ4, R, WR, WK, false, false>(a, own, blockIdx.x - before, lds);
+        if ((int)blockIdx.x < before) attend_chunk<NB, KQ4, VQ4, RP, true, false>(a, pre, blockIdx.x, lds);
+        else attend_chunk<NB, KQ4, VQ4, R, false, false>(a, own, blockIdx.x - before, lds);
     } else {
-        attend_chunk<NB, KQ4, VQ4, R, WR, WK, false, R == 1 && WK == 4>(a, own, blockIdx.x, lds);
+        attend_chunk<NB, KQ4, VQ4, R, false, R == 1>(a, own, blockIdx.x, lds);
     }
 }
 
@@ -693,55 +714,46 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
 }
 
 // ---- host ----
-struct Config {
-    int r, wr, wk;
-};
 constexpr int PRE_R = 2;
 constexpr int TARGET = 512;        // workgroups: two per CU
 constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (25.0 us against 27.6 at 512)
 constexpr size_t ARRIVED_BYTES = (size_t)4 * TARGET * COUNTER_STRIDE;   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
-    Config own_cfg;
     Plan own{}, pre{};
-    int groups;            // workgroups of the own part, per kv head
-    bool fused;
+    int r;                 // tiles of a wavefront
+    bool fused;            // chunks joined by the workgroup that finishes last
     size_t bytes = 0;
 };
 
 int rows_per_wave(int blocks) { return blocks == 8 ? 1 : 2; }   // tiles of 16: registers for two wavefronts per SIMD
 
 // Shapes of the launch, from sizes that the host knows (lengths are on the
-// device).  16 rows or fewer (decode): four wavefronts share the keys of one
-// tile.  More: one tile of 32 rows per workgroup, its keys over the wavefronts
-// and, in chunks, over workgroups; where prompts are so long that pairs of 128
-// rows give a workgroup for every CU, four wavefronts of 32 rows each walk the
-// same keys (not at head_dim 256, whose tiles leave no registers for two
-// wavefronts per SIMD).
+// device).  16 rows or fewer of a kv head and sequence (decode): tiles of 16
+// rows, more: of 32 (16 at head_dim 256, whose tiles leave no registers for
+// two wavefronts per SIMD).  A tile's keys go over the wavefronts of its
+// workgroup and, where tiles are too few for the card, in chunks over several.
 Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len, uint8_t* work) {
     Plans p;
     const int group = heads / c.kv_heads, r = rows_per_wave(c.head_dim / 32);
     const int64_t rows = (int64_t)tokens * group, want = TARGET / c.kv_heads;
     auto tiles_of = [](int64_t n, int per) { return (int)((n + per - 1) / per); };
-    if (rows <= 16) p.own_cfg = {1, 1, 4};
-    else if (!prefix && r == 2 && (int64_t)batch * tiles_of(rows, 128 * r) * c.kv_heads >= TARGET / 2) p.own_cfg = {r, 4, 1};
-    else p.own_cfg = {r, 1, 4};
+    p.r = rows <= 16 ? 1 : r;
     Plan& o = p.own;
-    o.rows = 16 * p.own_cfg.r * p.own_cfg.wr;
+    o.rows = 16 * p.r;
     o.tiles = tiles_of(rows, o.rows);
     o.entries = batch * o.tiles;
-    // two records a wavefront pay for a chunk's own time (4096 keys of the 7B shape: 10.8 us, at one 12.6)
-    o.least = 2 * p.own_cfg.wk;
+    // two records a wavefront pay for a chunk's own time (4096 keys of the 7B shape: 10.0 us, at one 11.7)
+    o.least = 2 * WAVES;
     o.per_record = 1.f / (float)o.least * (1.f - 0x1p-18f);
     o.by_tiles = Divisor(o.tiles);
     o.by_batch = Divisor(batch);
     const int64_t most = tiles_of(c.groups, o.least);   // chunks of an entry
     o.items = o.entries;
-    if (p.own_cfg.wk > 1 && o.entries < want && most > 1)
+    if (o.entries < want && most > 1)
         o.items = (int)std::max<int64_t>(std::min(want, o.entries * (most + 1)), o.entries * 3 / 2 + 1);
-    p.groups = p.own_cfg.wk > 1 ? o.items : batch * tiles_of(o.tiles, 2);
     o.whole = o.items == o.entries ? prefix ? 2 : 1 : 0;
-    p.fused = !prefix && p.own_cfg.r == 1 && p.own_cfg.wk == 4 && !o.whole;
+    p.fused = !prefix && p.r == 1 && !o.whole;
     size_t at = 0;
     auto take = [&](size_t n) {
         uint8_t* q = work + at;
@@ -773,13 +785,9 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
 
 template <int NB, bool KQ4, bool VQ4, int RP>
 void launch_own(const Plans& p, const KvAttnArgs& a, hipStream_t s) {
-    const dim3 grid((uint32_t)((p.groups + p.pre.items) * a.cache.kv_heads));
-    constexpr int R = NB == 8 ? 1 : 2;
-    const Config& f = p.own_cfg;
-    if (a.rows.tokens * (a.heads / a.cache.kv_heads) <= 16)
-        kv_attention_kernel<NB, KQ4, VQ4, 1, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
-    else if (f.wr == 1) kv_attention_kernel<NB, KQ4, VQ4, R, 1, 4, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
-    else if constexpr (RP == 0 && R == 2) kv_attention_kernel<NB, KQ4, VQ4, R, 4, 1, 0><<<grid, 2 * THREADS, 0, s>>>(a, p.own, p.pre);
+    const dim3 grid((uint32_t)((p.own.items + p.pre.items) * a.cache.kv_heads));
+    if (p.r == 1) kv_attention_kernel<NB, KQ4, VQ4, 1, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
+    else kv_attention_kernel<NB, KQ4, VQ4, NB == 8 ? 1 : 2, RP><<<grid, THREADS, 0, s>>>(a, p.own, p.pre);
 }
 
 template <int NB, bool KQ4, bool VQ4>

@@ -39,17 +39,19 @@ def attend(q, k, v, first, window=0, scale=None):
     group = heads // k.shape[1]
     scale = scale or 1.0 / math.sqrt(hd)
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
-    for i in range(n):
-        end = first + i + 1
-        low = max(0, end - window) if window else 0
-        for h in range(heads):
-            kk, vv = k[low:end, h // group], v[low:end, h // group]
-            s = (kk @ q[i, h].astype(np.float64)) * scale
-            e = np.exp(s - s.max())
-            out[i, h] = (e @ vv) / e.sum()
-            mag = (np.abs(kk) @ np.abs(q[i, h].astype(np.float64))).max() * scale
-            off = (hd + 16) * U * mag + 16 * U + 6 * U * np.abs(s).max()
-            tol[i, h] = 2 * np.abs(vv).max() * (off + 8 * U + (end - low) * U)
+    at, key = first + np.arange(n)[:, None], np.arange(k.shape[0])[None, :]
+    seen = (key <= at) & (key > at - window) if window else key <= at
+    count = seen.sum(-1)
+    for h in range(heads):
+        kk, vv, qq = k[:, h // group], v[:, h // group], q[:, h].astype(np.float64)
+        s = np.where(seen, (qq @ kk.T) * scale, -np.inf)
+        e = np.exp(s - s.max(-1, keepdims=True))
+        out[:, h] = (e @ vv) / e.sum(-1, keepdims=True)
+        mag = np.where(seen, np.abs(qq) @ np.abs(kk).T, 0.0).max(-1) * scale
+        most = np.where(seen, np.abs(s), 0.0).max(-1)
+        off = (hd + 16) * U * mag + 16 * U + 6 * U * most
+        vmax = np.where(seen, np.abs(vv).max(-1)[None, :], 0.0).max(-1)
+        tol[:, h] = (2 * vmax * (off + 8 * U + count * U))[:, None]
     return out, tol
 
 

@@ -105,6 +105,25 @@ def test_prompts(hip, head_dim, kv_heads, group, tokens):
     case.check(kv_heads * group, tokens, [0, 61])
 
 
+@pytest.mark.parametrize("head_dim,kv_heads,group,types", [(64, 8, 8, (Q8_0, Q4_0)), (96, 32, 1, (Q4_0, Q8_0)),
+                                                           (128, 8, 4, (Q8_0, Q8_0)), (128, 8, 5, (Q4_0, Q4_0)),
+                                                           (256, 4, 2, (Q8_0, Q8_0))])
+def test_prompts_that_fill_the_card(hip, head_dim, kv_heads, group, types):
+    """So many rows that tiles of 128 go in pairs (not at head_dim 256): an odd number of tiles, ragged prompts, one
+    empty, some behind a history, a window."""
+    tokens = 256 * 3 // group + 11
+    batch = -(-256 // (kv_heads * 4)) + 1
+    lengths = [tokens + 17 * b for b in range(batch)]
+    starts = [17 * b for b in range(batch)]
+    counts = [max(0, tokens - 60 * b) for b in range(batch)]
+    if batch > 2:
+        counts[2] = 0
+    counts[1] = 1
+    case = Case(hip, kv_heads, head_dim, lengths, types, seed=head_dim + group)
+    case.check(kv_heads * group, tokens, starts, counts)
+    case.check(kv_heads * group, tokens, starts, counts, window=45)
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 100, 250, 5000])
 @pytest.mark.parametrize("prefix", [0, 150])
 def test_window(hip, window, prefix):
