@@ -57,7 +57,7 @@ internal static unsafe partial class HipNative
         public float Eps;
         public float RopeBase;
         public float RopeLinearFactor;
-        public int KvFp16;
+        public int KvFp16;        // 1 fp16, 0 fp32; 2 and 3: quantised to Q8_0 and Q4_0
         public int Bos;
         public int SlidingWindow; // attend to the last N positions (IE:385-387); 0 = all
         public byte* KeyPrefix;   // NUL-terminated UTF-8, may be null

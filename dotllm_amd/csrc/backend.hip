@@ -937,6 +937,11 @@ struct llmdot_hip_model {
     // KV cache [layer][kv_head][context][head_dim]
     uint8_t *kcache = nullptr, *vcache = nullptr;
     size_t kv_layer_bytes = 0;
+    // quantised instead (kv_quantised): one slot per layer, kvq.k the allocation;
+    // layer_ids[l] = l, and the attention's workspaces
+    KvView kvq{};
+    int32_t* layer_ids = nullptr;
+    uint8_t *kvq_work = nullptr, *pf_kvq_work = nullptr;   // single tokens; prompt chunks
     float *cos_tab = nullptr, *sin_tab = nullptr;
     int rope_half = 0;
     // attention scratch
@@ -985,6 +990,9 @@ namespace {
 int32_t* m_token(llmdot_hip_model* m) { return m->ints; }
 int32_t* m_pos(llmdot_hip_model* m) { return m->ints + 1; }
 int32_t* m_step(llmdot_hip_model* m) { return m->ints + 2; }
+// first position of the prompt chunk or cache row at hand (quantised cache)
+int32_t* m_start(llmdot_hip_model* m) { return m->ints + 5; }
+bool kv_quantised(const llmdot_hip_model_desc& d) { return d.kv_fp16 == LLMDOT_KV_Q8_0 || d.kv_fp16 == LLMDOT_KV_Q4_0; }
 uint32_t* m_epoch(llmdot_hip_model* m) { return reinterpret_cast<uint32_t*>(m->ints + 3); }
 int32_t* m_err(llmdot_hip_model* m) { return m->ints + 4; }
 
@@ -1068,6 +1076,27 @@ int enqueue_head(llmdot_hip_model* m) {
     return 0;
 }
 
+// Layer l's attention over the quantised cache for T tokens at positions *start
+// ..: the projections in aa (q, k and v, or their parts) rotated, k and v
+// written, then out.  q, k and v receive the rotated rows.
+int enqueue_quantised_attention(llmdot_hip_model* m, int l, const PfAttnArgs& aa, const int32_t* start, float* q, float* k,
+                                float* v, float* out) {
+    const auto& d = m->d;
+    hipStream_t s = m->ctx->stream;
+    HIPCHK(launch_rope_rows(aa, start, q, k, v, s));
+    const KvRows rows{1, aa.T, m->layer_ids + l, start, nullptr};
+    const int64_t kvdim = (int64_t)d.kv_heads * d.head_dim, qdim = (int64_t)d.heads * d.head_dim;
+    HIPCHK(launch_kv_write(m->kvq, rows, k, kvdim, v, kvdim, s));
+    KvAttnArgs at{};
+    at.cache = m->kvq; at.rows = rows;
+    at.q = q; at.out = out; at.q_stride = at.out_stride = qdim;
+    at.heads = d.heads; at.window = d.sliding_window;
+    at.scale = 1.0f / sqrtf((float)d.head_dim);
+    at.work = aa.T == 1 ? m->kvq_work : m->pf_kvq_work;
+    HIPCHK(launch_kv_attention(at, s));
+    return 0;
+}
+
 // Enqueues one decode step on the model stream (token and position on the device).
 int enqueue_step(llmdot_hip_model* m) {
     const auto& d = m->d;
@@ -1107,6 +1136,14 @@ int enqueue_step(llmdot_hip_model* m) {
         }
         if (w.q_norm_f || w.k_norm_f)   // per-head Q/K RmsNorm before RoPE (IE:354-359, IE:367-372)
             HIPCHK(launch_qk_norm(m->q, m->k, w.q_norm_f, w.k_norm_f, d.heads, d.kv_heads, d.head_dim, d.eps, s));
+        if (kv_quantised(d)) {
+            PfAttnArgs pa{};
+            pa.q = m->q; pa.k = m->k; pa.v = m->v;
+            pa.q_split = pa.k_split = pa.v_split = 1;
+            pa.cos_tab = m->cos_tab; pa.sin_tab = m->sin_tab;
+            pa.T = 1; pa.heads = d.heads; pa.kv_heads = d.kv_heads; pa.head_dim = d.head_dim; pa.rope_half = m->rope_half;
+            if (int rc = enqueue_quantised_attention(m, l, pa, m_pos(m), m->q, m->k, m->v, m->attn)) return rc;
+        }
         AttnArgs aa{};
         aa.q = m->q; aa.k = m->k; aa.v = m->v;
         aa.kcache = m->kcache + (size_t)l * m->kv_layer_bytes;
@@ -1120,7 +1157,7 @@ int enqueue_step(llmdot_hip_model* m) {
         aa.layer = l; aa.layers = d.layers; aa.spin_max = m->attn_spin; aa.err = m_err(m);
         aa.xcd_exchange = m->attn_xcd_exchange ? 1 : 0; aa.xpart = m->xpart;
         aa.window = d.sliding_window;
-        HIPCHK(launch_attention(aa, s));
+        if (!kv_quantised(d)) HIPCHK(launch_attention(aa, s));
         {   // O projection + residual (IE:444-449, IE:189), h packed for the FFN RmsNorm
             GemvArgs ga{};
             ga.nseg = 1; ga.seg[0] = {w.o->dev, nullptr, m->h, d.hidden, 0};
@@ -1234,6 +1271,10 @@ int ensure_prefill_ws(llmdot_hip_model* m) {
     if ((rc = A(2 * cap * (kmax / 32), &p))) return rc; m->pf_planes.sl = (_Float16*)p;
     if ((rc = A(4 * (size_t)cap, &p))) return rc; m->pf_planes.xinv = (float*)p;
     if ((rc = A(4 * (size_t)cap, &p))) return rc; m->pf_tokens = (int32_t*)p;
+    if (kv_quantised(d)) {
+        if ((rc = A(kv_attention_workspace_upto(m->kvq, d.heads, cap), &p))) return rc;
+        m->pf_kvq_work = (uint8_t*)p;
+    }
     m->pf_cap = cap;
     return 0;
 }
@@ -1318,13 +1359,17 @@ int enqueue_prefill_chunk(llmdot_hip_model* m, int T, int pos0) {
         aa.context = d.context; aa.kv_fp16 = d.kv_fp16;
         aa.q_norm = w.q_norm_f; aa.k_norm = w.k_norm_f; aa.eps = d.eps;
         aa.window = d.sliding_window;
-        HIPCHK(launch_prefill_rope_kv(aa, s));
+        if (kv_quantised(d)) {
+            if (int rc = enqueue_quantised_attention(m, l, aa, m_start(m), m->pf_qr, m->pf_k, m->pf_v, m->pf_attn)) return rc;
+        } else {
+            HIPCHK(launch_prefill_rope_kv(aa, s));
+        }
         // the projections' parts are summed: their buffers take the splits'
         aa.splits = prefill_attn_splits(T, pos0, d.heads, d.kv_fp16, d.sliding_window);
         aa.part_out = m->pf_parts_q; aa.part_z = m->pf_parts_k; aa.part_max = m->pf_parts_v;
         aa.part_stride = (int64_t)T * qdim;
-        if (aa.splits * aa.part_stride > PF_PARTS_MAX) aa.splits = 1;
-        HIPCHK(launch_prefill_attention(aa, s));
+        if (aa.splits * aa.part_stride > PF_PARTS_MAX || kv_quantised(d)) aa.splits = 1;
+        if (!kv_quantised(d)) HIPCHK(launch_prefill_attention(aa, s));
         if (aa.splits > 1) HIPCHK(launch_prefill_planes_attn(aa, pl, s));
         else HIPCHK(launch_prefill_planes(m->pf_attn, T, qdim, nullptr, 0.f, pl, s));
         HIPCHK(proj_add(w.o, qdim));
@@ -1364,6 +1409,7 @@ int prefill_batched(llmdot_hip_model* m, const int32_t* tokens, int n, int pos0,
     for (int c0 = 0; c0 < n; c0 += m->pf_cap) {
         T = std::min(m->pf_cap, n - c0);
         if (int rc = send(m->ctx, m->pf_tokens, tokens + c0, sizeof(int32_t) * (size_t)T)) return rc;
+        if (int rc = set_int(m, m_start(m), pos0 + c0)) return rc;
         if (int rc = enqueue_prefill_chunk(m, T, pos0 + c0)) return rc;
     }
     const float* h_last = m->pf_h + (size_t)(T - 1) * m->d.hidden;
@@ -1533,10 +1579,23 @@ extern "C" int32_t llmdot_hip_model_create(llmdot_hip_ctx* ctx, const llmdot_hip
     if ((rc = A(sizeof(float) * d.hidden, &p))) return bail(rc); m->xn = (float*)p;
     if ((rc = A(sizeof(float) * (d.hidden / 4), &p))) return bail(rc); m->xssq = (float*)p;
     if ((rc = A(sizeof(float) * d.vocab, &p))) return bail(rc); m->logits = (float*)p;
-    const size_t elt = d.kv_fp16 ? 2 : 4;
-    m->kv_layer_bytes = (size_t)d.kv_heads * d.context * d.head_dim * elt;
-    if ((rc = A(m->kv_layer_bytes * d.layers, &p))) return bail(rc); m->kcache = (uint8_t*)p;
-    if ((rc = A(m->kv_layer_bytes * d.layers, &p))) return bail(rc); m->vcache = (uint8_t*)p;
+    if (kv_quantised(d)) {
+        const bool q4 = d.kv_fp16 == LLMDOT_KV_Q4_0;
+        m->kvq = kv_view(d.layers, d.kv_heads, d.head_dim, d.context, q4, q4);
+        const size_t records = (size_t)d.layers * d.kv_heads * m->kvq.groups;
+        if ((rc = A(records * m->kvq.k_rec, &p))) return bail(rc); m->kvq.k = (uint8_t*)p;
+        if ((rc = A(records * m->kvq.v_rec, &p))) return bail(rc); m->kvq.v = (uint8_t*)p;
+        if ((rc = A(kv_attention_workspace(m->kvq, d.heads, 1, 1, false), &p))) return bail(rc); m->kvq_work = (uint8_t*)p;
+        std::vector<int32_t> ids((size_t)d.layers);
+        for (int l = 0; l < d.layers; l++) ids[(size_t)l] = l;
+        if ((rc = A(4 * ids.size(), &p)) || (rc = copy_in(ctx, p, ids.data(), 4 * ids.size()))) return bail(rc);
+        m->layer_ids = (int32_t*)p;
+    } else {
+        const size_t elt = d.kv_fp16 ? 2 : 4;
+        m->kv_layer_bytes = (size_t)d.kv_heads * d.context * d.head_dim * elt;
+        if ((rc = A(m->kv_layer_bytes * d.layers, &p))) return bail(rc); m->kcache = (uint8_t*)p;
+        if ((rc = A(m->kv_layer_bytes * d.layers, &p))) return bail(rc); m->vcache = (uint8_t*)p;
+    }
     const int nch = attn_max_chunks(d.heads, d.kv_heads, d.context);
     if ((rc = A(sizeof(float) * (size_t)d.heads * d.context, &p))) return bail(rc); m->scores = (float*)p;
     if ((rc = A(sizeof(float) * (size_t)d.heads * nch, &p))) return bail(rc); m->chunk_max = (float*)p;
@@ -1546,7 +1605,7 @@ extern "C" int32_t llmdot_hip_model_create(llmdot_hip_ctx* ctx, const llmdot_hip
     if (const char* v = getenv("LLMDOT_HIP_ATTN_FUSED")) m->attn_fused = m->attn_fused && strcmp(v, "0") != 0;
     if (const char* v = getenv("LLMDOT_HIP_ATTN_SPIN")) m->attn_spin = atoi(v) >= 0 ? atoi(v) : m->attn_spin;
     if (d.sliding_window < 0) return bail(fail(LLMDOT_E_INVALID, "negative sliding window"));
-    if (d.sliding_window > 0 && !m->attn_fused)
+    if (d.sliding_window > 0 && !m->attn_fused && !kv_quantised(d))
         return bail(fail(LLMDOT_E_UNSUPPORTED, "sliding-window attention needs the one-launch attention "
                                                "(at most 16384 positions, LLMDOT_HIP_ATTN_FUSED not 0)"));
     if ((rc = A(sizeof(uint64_t) * (size_t)attn_xmax_slots(d.heads), &p))) return bail(rc); m->xmax = (uint64_t*)p;
@@ -1557,7 +1616,7 @@ extern "C" int32_t llmdot_hip_model_create(llmdot_hip_ctx* ctx, const llmdot_hip
         const char* v = getenv("LLMDOT_HIP_ATTN_XCD");
         int cus = 0;
         HIPCHK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, m->ctx->device));
-        bool want = m->attn_fused && !(v && strcmp(v, "0") == 0) &&
+        bool want = m->attn_fused && !kv_quantised(d) && !(v && strcmp(v, "0") == 0) &&
                     attn_xcd_fits(d.heads, d.kv_heads, d.head_dim, d.context, d.kv_fp16 ? 1 : 0, cus);
         if (want) {
             bool ok = false;
@@ -1847,6 +1906,16 @@ extern "C" int32_t llmdot_hip_kv_read(llmdot_hip_model* m, int32_t layer, int32_
     if (layer < 0 || layer >= m->d.layers) return fail(LLMDOT_E_RANGE, "layer out of range");
     if (int rc = check_pos(m, position)) return rc;
     const auto& d = m->d;
+    if (kv_quantised(d)) {   // through the step's k and v rows, which hold nothing between steps
+        const size_t n = sizeof(float) * (size_t)d.kv_heads * d.head_dim;
+        if (int rc = set_int(m, m_start(m), position)) return rc;
+        const KvRows rows{1, 1, m->layer_ids + layer, m_start(m), nullptr};
+        const int64_t stride = (int64_t)d.kv_heads * d.head_dim;
+        HIPCHK(launch_kv_read(m->kvq, rows, m->k, stride, m->v, stride, m->ctx->stream));
+        HIPCHK(hipMemcpyAsync(k, m->k, n, hipMemcpyDeviceToHost, m->ctx->stream));
+        HIPCHK(hipMemcpyAsync(v, m->v, n, hipMemcpyDeviceToHost, m->ctx->stream));
+        return wait_stream(m->ctx);
+    }
     const size_t elt = d.kv_fp16 ? 2 : 4;
     std::vector<uint8_t> kb((size_t)d.head_dim * elt), vb((size_t)d.head_dim * elt);
     if (int rc = wait_stream(m->ctx)) return rc;
@@ -1881,7 +1950,7 @@ extern "C" int32_t llmdot_hip_model_step_bytes(llmdot_hip_model* m, int32_t posi
     }
     b += (double)m->out->nbytes + (double)m->out_norm->nbytes;
     b += (double)byte_count(m->embd->type, d.hidden);
-    const double elt = d.kv_fp16 ? 2.0 : 4.0;
+    const double elt = d.kv_fp16 == LLMDOT_KV_Q8_0 ? 34.0 / 32 : d.kv_fp16 == LLMDOT_KV_Q4_0 ? 18.0 / 32 : d.kv_fp16 ? 2.0 : 4.0;
     b += (double)d.layers * 2.0 * (double)(position + 1) * (double)(d.kv_heads * d.head_dim) * elt;
     *bytes = b;
     return 0;
@@ -1892,6 +1961,7 @@ extern "C" int32_t llmdot_hip_model_kv_fill_random(llmdot_hip_model* m, int32_t 
     m->gen.active = false;
     if (n < 0 || n > m->d.context) return fail(LLMDOT_E_RANGE, "fill length outside the KV cache");
     const auto& d = m->d;
+    if (kv_quantised(d)) return fail(LLMDOT_E_UNSUPPORTED, "a quantised KV cache has no seeded fill");
     HIPCHK(launch_kv_fill(m->kcache, 0, d.layers, d.kv_heads, d.context, d.head_dim, n, seed, d.kv_fp16, m->ctx->stream));
     HIPCHK(launch_kv_fill(m->vcache, 1, d.layers, d.kv_heads, d.context, d.head_dim, n, seed, d.kv_fp16, m->ctx->stream));
     if (int rc = wait_stream(m->ctx)) return rc;

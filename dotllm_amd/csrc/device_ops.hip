@@ -119,12 +119,7 @@ extern "C" int32_t llmdot_hip_kv_cache_create(llmdot_hip_ctx* ctx, const llmdot_
         for (uint32_t t : {d.k_type, d.v_type})
             if (t != GGML_Q8_0 && t != GGML_Q4_0)
                 return ctx_fail(LLMDOT_E_UNSUPPORTED, "KV cache type " + std::to_string(t) + " is not Q8_0 or Q4_0");
-        KvView v{};
-        v.slots = d.slots; v.kv_heads = d.kv_heads; v.head_dim = d.head_dim; v.capacity = d.capacity;
-        v.groups = (d.capacity + KV_GROUP - 1) / KV_GROUP;
-        v.k_q4 = d.k_type == GGML_Q4_0; v.v_q4 = d.v_type == GGML_Q4_0;
-        v.k_rec = kv_record_bytes(v.k_q4, d.head_dim / 32, false);
-        v.v_rec = kv_record_bytes(v.v_q4, d.head_dim / 32, true);
+        KvView v = kv_view(d.slots, d.kv_heads, d.head_dim, d.capacity, d.k_type == GGML_Q4_0, d.v_type == GGML_Q4_0);
         const double records = (double)d.slots * d.kv_heads * v.groups;
         if (records * (v.k_rec + v.v_rec) > 1e15) return ctx_fail(LLMDOT_E_NOMEM, "KV cache too large");
         const size_t kb = (size_t)records * v.k_rec, vb = (size_t)records * v.v_rec;

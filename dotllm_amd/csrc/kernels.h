@@ -297,6 +297,12 @@ hipError_t launch_prefill_rope_kv(const PfAttnArgs& a, hipStream_t s);
 hipError_t launch_prefill_attention(const PfAttnArgs& a, hipStream_t s);
 // prefill_attn.hip: the same with 16 queries per workgroup, its wavefronts over the keys.
 hipError_t launch_prefill_attn_wave(const PfAttnArgs& a, hipStream_t s);
+// A layer's projections of T tokens at positions *start .. on their way to a
+// quantised KV cache: sums of their K parts, per-head norms (where given), RoPE,
+// as fp32 rows q_out [T][heads * head_dim], k_out and v_out [T][kv_heads *
+// head_dim] (in place of an input that is one part).
+hipError_t launch_rope_rows(const PfAttnArgs& a, const int32_t* start, float* q_out, float* k_out, float* v_out,
+                            hipStream_t s);
 // Embedding rows tokens[0..T) (device ids) into out[T][hidden].
 hipError_t launch_embed_rows(const uint8_t* table, uint32_t type, int hidden, const int32_t* tokens, int T, float* out,
                              hipStream_t s);
@@ -326,6 +332,10 @@ struct KvAttnArgs {
 bool kv_attention_supported(int head_dim);
 size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix);
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s);
+// The most that calls of one sequence and 1 .. tokens tokens need.
+size_t kv_attention_workspace_upto(const KvView& c, int heads, int tokens);
+// A cache's shape; its two allocations hold slots * kv_heads * groups records each.
+KvView kv_view(int slots, int kv_heads, int head_dim, int capacity, bool k_q4, bool v_q4);
 
 // ---- verify.hip (verification of drafted tokens) ----
 constexpr int VERIFY_BATCH = 4096;   // sequences of a call, at most

@@ -821,6 +821,12 @@ size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens,
     return make_plans(c, heads, batch, tokens, prefix, -1, nullptr).bytes;
 }
 
+size_t kv_attention_workspace_upto(const KvView& c, int heads, int tokens) {
+    size_t most = 0;
+    for (int t = 1; t <= tokens; t++) most = std::max(most, kv_attention_workspace(c, heads, 1, t, false));
+    return most;
+}
+
 hipError_t launch_kv_attention(const KvAttnArgs& a, hipStream_t s) {
     switch (a.cache.head_dim) {
         case 64: return launch_blocks<2>(a, s);

@@ -265,6 +265,44 @@ __global__ __launch_bounds__(THREADS) void kv_read_kernel(KvView c, KvRows rows,
     }
 }
 
+// One wavefront per head row of a token (q heads, then k, then v).
+__global__ __launch_bounds__(64) void rope_rows_kernel(PfAttnArgs a, const int32_t* start, float* q_out, float* k_out,
+                                                       float* v_out) {
+    const int hd = a.head_dim, t = blockIdx.x, lane = threadIdx.x, half = a.rope_half;
+    int h = blockIdx.y;
+    const float *in = a.q, *norm = a.q_norm;
+    float* out = q_out;
+    int split = a.q_split, heads = a.heads;
+    int64_t part = a.q_part;
+    bool turns = true;
+    if (h >= a.heads + a.kv_heads) {
+        h -= a.heads + a.kv_heads;
+        in = a.v; norm = nullptr; out = v_out; split = a.v_split; part = a.v_part; heads = a.kv_heads; turns = false;
+    } else if (h >= a.heads) {
+        h -= a.heads;
+        in = a.k; norm = a.k_norm; out = k_out; split = a.k_split; part = a.k_part; heads = a.kv_heads;
+    }
+    const int64_t row = ((int64_t)t * heads + h) * hd;
+    __shared__ float x[256];
+    float ss = 0.f;
+    for (int d = lane; d < hd; d += 64) {
+        float v = in[row + d];
+        for (int p = 1; p < split; p++) v += in[row + p * part + d];
+        x[d] = v;
+        ss += v * v;
+    }
+    if (norm) {
+        const float inv = 1.f / sqrtf(wave_sum(ss) / (float)hd + a.eps);
+        for (int d = lane; d < hd; d += 64) x[d] = norm[d] * x[d] * inv;
+    }
+    __syncthreads();
+    const int64_t pos = *start + t;
+    for (int d = lane; d < hd; d += 64) {
+        const int64_t c = pos * half;
+        out[row + d] = turns ? rope_elem(x, d, half, a.cos_tab + c, a.sin_tab + c) : x[d];
+    }
+}
+
 // Records that a run of `tokens` positions can touch.
 int run_groups(int tokens, const KvView& c) {
     const int64_t n = ((int64_t)tokens + KV_GROUP - 2) / KV_GROUP + 1;
@@ -292,6 +330,23 @@ hipError_t for_shape(const KvView& c, F&& f) {
 }
 
 }  // namespace
+
+hipError_t launch_rope_rows(const PfAttnArgs& a, const int32_t* start, float* q_out, float* k_out, float* v_out,
+                            hipStream_t s) {
+    if (a.T <= 0 || a.head_dim > 256) return hipErrorInvalidValue;
+    rope_rows_kernel<<<dim3(a.T, a.heads + 2 * a.kv_heads), 64, 0, s>>>(a, start, q_out, k_out, v_out);
+    return hipGetLastError();
+}
+
+KvView kv_view(int slots, int kv_heads, int head_dim, int capacity, bool k_q4, bool v_q4) {
+    KvView v{};
+    v.slots = slots; v.kv_heads = kv_heads; v.head_dim = head_dim; v.capacity = capacity;
+    v.groups = (capacity + KV_GROUP - 1) / KV_GROUP;
+    v.k_q4 = k_q4; v.v_q4 = v_q4;
+    v.k_rec = kv_record_bytes(k_q4, head_dim / 32, false);
+    v.v_rec = kv_record_bytes(v_q4, head_dim / 32, true);
+    return v;
+}
 
 hipError_t launch_kv_write(const KvView& c, const KvRows& rows, const float* k, int64_t ks, const float* v, int64_t vs,
                            hipStream_t s) {

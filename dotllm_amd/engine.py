@@ -51,6 +51,10 @@ LAYER_TENSORS = ("attn_norm", "attn_q", "attn_k", "attn_v", "attn_qkv", "attn_q_
                  "ffn_norm", "ffn_gate", "ffn_up", "ffn_down")
 
 
+# KV cache element types (llmdot_hip_model_desc.kv_fp16).
+KV_TYPES = {"f32": 0, "f16": 1, "q8_0": 2, "q4_0": 3}
+
+
 class LoadedModel:
     """A parsed GGUF model (tensors are zero-copy views of the file or image).
 
@@ -95,7 +99,11 @@ class InferenceEngine:
     """Greedy decode of a LLaMA-like GGUF model on one MI355X."""
 
     def __init__(self, model: LoadedModel, backend: HipBackend | None = None, *, kv_fp16: bool = True,
-                 context: int | None = None):
+                 context: int | None = None, kv_type: str | None = None):
+        """kv_type: the KV cache's element type, "f32" (the reference's), "f16", "q8_0" or "q4_0" (quantised as
+        rows are written, see kvcache.KvCache); None goes by kv_fp16."""
+        if kv_type is not None and kv_type not in KV_TYPES:
+            raise ValueError(f"kv_type must be one of {', '.join(KV_TYPES)}")
         cfg = model.config
         if cfg.ffn_type != "swiglu":
             raise NotImplementedError("only SwiGLU FFN tensors are supported")
@@ -120,7 +128,7 @@ class InferenceEngine:
         d.eps, d.rope_base = cfg.norm_epsilon, cfg.rope_freq_base
         d.rope_linear_factor = (cfg.rope_scaling_factor
                                 if cfg.rope_scaling_type == "linear" and cfg.rope_scaling_factor > 1 else 1.0)
-        d.kv_fp16 = 1 if kv_fp16 else 0
+        d.kv_fp16 = KV_TYPES[kv_type] if kv_type is not None else 1 if kv_fp16 else 0
         d.bos = cfg.bos_token_id
         d.sliding_window = int(cfg.sliding_window)
         d.key_prefix = prefix.encode()

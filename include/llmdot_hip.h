@@ -189,6 +189,8 @@ int32_t llmdot_hip_stream_bench(llmdot_hip_ctx* ctx, size_t nbytes, int32_t mode
 
 /* ---- model level: the device-resident decode step (InferenceEngine.ProcessToken,
  *      IE:134-146, LLaMA-like template IE:184-196) and greedy Generate (IE:74-132). */
+#define LLMDOT_KV_Q8_0 2
+#define LLMDOT_KV_Q4_0 3
 typedef struct llmdot_hip_model_desc {
     int32_t hidden;          /* TransformerConfig.HiddenSize          */
     int32_t layers;          /* LayerCount                            */
@@ -202,7 +204,9 @@ typedef struct llmdot_hip_model_desc {
     float eps;               /* NormEpsilon                           */
     float rope_base;         /* RopeFreqBase                          */
     float rope_linear_factor;/* RopeScalingFactor when type is Linear, else 1 */
-    int32_t kv_fp16;         /* 1: fp16 KV cache (default), 0: fp32 as the reference */
+    int32_t kv_fp16;         /* 1: fp16 KV cache (default), 0: fp32 as the reference;
+                              * LLMDOT_KV_Q8_0, LLMDOT_KV_Q4_0: quantised as llmdot_hip_cache.h
+                              * describes (with the exact exponential in its softmax) */
     int32_t bos;             /* BosTokenId (used when the prompt is empty) */
     int32_t sliding_window;  /* SlidingWindow: attend to the last N positions (IE:385-387); 0 = all */
     /* Weight keys follow GGUF tensor names (src/Llmdot.Core/Loading/TensorNameResolver.cs:22-107):
@@ -306,8 +310,9 @@ int32_t llmdot_hip_model_step_bytes(llmdot_hip_model* model, int32_t position, d
  * the K (kind 0) or V (kind 1) row of (layer, pos) is
  *   key = (2 layer + kind) << 44 | pos << 20 | e,  z = SplitMix64 finaliser of
  *   seed + 0x9E3779B97F4A7C15 (key + 1),  value = ((z >> 40) / 2^24 - 0.5) * 3,
- * stored in the cache's element type (fp16: round to nearest even).  No
- * reference counterpart: a test and timing aid. */
+ * stored in the cache's element type (fp16: round to nearest even;
+ * LLMDOT_E_UNSUPPORTED for a quantised cache).  No reference counterpart: a
+ * test and timing aid. */
 int32_t llmdot_hip_model_kv_fill_random(llmdot_hip_model* model, int32_t n, uint64_t seed);
 
 /* ---- GGUF tooling: reference-layout quantizers and seeded synthetic weights
