@@ -39,12 +39,14 @@ int device_error(const char* what, hipError_t e) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// The call's rows, checked; *total = batch * tokens.
+// The call's rows, checked; *total = batch * tokens.  A call of none is checked for
+// its sizes only: empty arrays have no address.
 int check_rows(const llmdot_hip_token_batch* rows, KvRows* out, int64_t* total) {
-    if (!rows || !rows->slots_dev || !rows->starts_dev) return ctx_fail(LLMDOT_E_INVALID, "null token batch");
+    if (!rows) return ctx_fail(LLMDOT_E_INVALID, "null token batch");
     if (rows->batch < 0 || rows->tokens < 0) return ctx_fail(LLMDOT_E_INVALID, "negative batch or tokens");
-    if (rows->batch > 4096) return ctx_fail(LLMDOT_E_UNSUPPORTED, "more than 4096 sequences in a call");
+    if (rows->batch > MAX_SEQUENCES) return ctx_fail(LLMDOT_E_UNSUPPORTED, "more than 4096 sequences in a call");
     *total = (int64_t)rows->batch * rows->tokens;
+    if (*total > 0 && (!rows->slots_dev || !rows->starts_dev)) return ctx_fail(LLMDOT_E_INVALID, "null slots or starts");
     *out = {rows->batch, rows->tokens, rows->slots_dev, rows->starts_dev, rows->counts_dev};
     return 0;
 }
@@ -84,12 +86,12 @@ int32_t move_rows(llmdot_hip_kv_cache* cache, T* k, int64_t ks, T* v, int64_t vs
     KvRows rows;
     int64_t total;
     if (int rc = check_rows(batch, &rows, &total)) return rc;
-    if (int rc = check_array("k", k)) return rc;
-    if (int rc = check_array("v", v)) return rc;
     const int64_t width = (int64_t)cache->view.kv_heads * cache->view.head_dim;
     if (int rc = check_stride("k", width, &ks)) return rc;
     if (int rc = check_stride("v", width, &vs)) return rc;
     if (total == 0) return 0;
+    if (int rc = check_array("k", k)) return rc;
+    if (int rc = check_array("v", v)) return rc;
     if (total * cache->view.kv_heads > MAX_GRID) return ctx_fail(LLMDOT_E_UNSUPPORTED, "too many rows in a call");
     OnDevice dev(ctx_device(cache->ctx));
     hipError_t e = dev.err;
@@ -193,7 +195,7 @@ extern "C" int32_t llmdot_hip_kv_cache_attention_workspace(const llmdot_hip_kv_c
     return guarded([&]() -> int32_t {
         if (!cache || !bytes) return ctx_fail(LLMDOT_E_INVALID, "null argument");
         if (batch < 0 || tokens < 0) return ctx_fail(LLMDOT_E_INVALID, "negative batch or tokens");
-        if (batch > 4096) return ctx_fail(LLMDOT_E_UNSUPPORTED, "more than 4096 sequences in a call");
+        if (batch > MAX_SEQUENCES) return ctx_fail(LLMDOT_E_UNSUPPORTED, "more than 4096 sequences in a call");
         if (int rc = check_attention_shape(cache, heads, (int64_t)batch * tokens)) return rc;
         *bytes = batch && tokens ? kv_attention_workspace(cache->view, heads, batch, tokens, has_prefix != 0) : 0;
         return 0;
@@ -208,8 +210,6 @@ extern "C" int32_t llmdot_hip_kv_cache_attention(llmdot_hip_kv_cache* cache, con
         KvAttnArgs a{};
         int64_t total;
         if (int rc = check_rows(rows, &a.rows, &total)) return rc;
-        if (int rc = check_array("q", q_dev)) return rc;
-        if (int rc = check_array("out", out_dev)) return rc;
         if (int rc = check_attention_shape(cache, opt->heads, total)) return rc;
         const KvView& v = cache->view;
         const int64_t width = (int64_t)opt->heads * v.head_dim;
@@ -230,6 +230,8 @@ extern "C" int32_t llmdot_hip_kv_cache_attention(llmdot_hip_kv_cache* cache, con
             a.prefix = p; a.prefix_slot = opt->prefix_slot; a.prefix_len = opt->prefix_len;
         }
         if (total == 0) return 0;
+        if (int rc = check_array("q", q_dev)) return rc;
+        if (int rc = check_array("out", out_dev)) return rc;
         const size_t need = kv_attention_workspace(v, opt->heads, a.rows.batch, a.rows.tokens, a.prefix_len > 0);
         if (need > 0) {
             if (int rc = check_array("workspace", workspace_dev)) return rc;
@@ -252,7 +254,7 @@ extern "C" int32_t llmdot_hip_kv_cache_attention(llmdot_hip_kv_cache* cache, con
 namespace {
 int check_verify_shape(int batch, int drafts, int vocab) {
     if (batch < 0 || drafts < 0 || vocab <= 0) return ctx_fail(LLMDOT_E_INVALID, "bad batch, drafts or vocabulary");
-    if (batch > VERIFY_BATCH || drafts > 1024 || vocab > (1 << 24))
+    if (batch > MAX_SEQUENCES || drafts > 1024 || vocab > (1 << 24))
         return ctx_fail(LLMDOT_E_UNSUPPORTED, "at most 4096 sequences, 1024 drafts and 2^24 tokens in a vocabulary");
     if ((int64_t)batch * (vocab / 1024 + 1) > MAX_GRID) return ctx_fail(LLMDOT_E_UNSUPPORTED, "too many logits in a call");
     return 0;
@@ -277,12 +279,12 @@ extern "C" int32_t llmdot_hip_verify_drafts(llmdot_hip_ctx* ctx, const float* ta
     return guarded([&]() -> int32_t {
         if (!ctx) return ctx_fail(LLMDOT_E_INVALID, "null ctx");
         if (int rc = check_verify_shape(batch, drafts, vocab)) return rc;
+        if (!(temperature <= 3e38f)) return ctx_fail(LLMDOT_E_INVALID, "temperature must be a number");
+        if (batch == 0) return 0;
         if (int rc = check_array("target", target_dev)) return rc;
         if (draft_dev && !aligned(draft_dev)) return ctx_fail(LLMDOT_E_INVALID, "draft is not 16-byte aligned");
         if ((drafts > 0 && !drafts_dev) || !uniforms_dev || !tokens_dev || !accepted_dev)
             return ctx_fail(LLMDOT_E_INVALID, "null argument");
-        if (!(temperature <= 3e38f)) return ctx_fail(LLMDOT_E_INVALID, "temperature must be a number");
-        if (batch == 0) return 0;
         const size_t need = verify_workspace(batch, drafts, vocab);
         if (need > 0) {
             if (int rc = check_array("workspace", workspace_dev)) return rc;

@@ -310,6 +310,10 @@ hipError_t launch_embed_rows(const uint8_t* table, uint32_t type, int hidden, co
 // Words between two arrival counters of a launch: atomics on one line of memory
 // wait for each other (about 14 ns each, whichever counter they are for).
 constexpr int COUNTER_STRIDE = 32;
+constexpr int MAX_SEQUENCES = 4096;   // of a call
+// Every workspace, of any operator, begins with counters that are zero between
+// launches: what one leaves there is fit for all others.
+constexpr size_t COUNTER_BYTES = sizeof(uint32_t) * MAX_SEQUENCES * COUNTER_STRIDE;
 
 // ---- kv_cache.hip, kv_attention.hip (quantised KV cache) ----
 // Rows of k and v [batch * tokens], ks and vs floats apart, into the cache, and back.
@@ -338,7 +342,6 @@ size_t kv_attention_workspace_upto(const KvView& c, int heads, int tokens);
 KvView kv_view(int slots, int kv_heads, int head_dim, int capacity, bool k_q4, bool v_q4);
 
 // ---- verify.hip (verification of drafted tokens) ----
-constexpr int VERIFY_BATCH = 4096;   // sequences of a call, at most
 struct VerifyArgs {
     const float *target, *draft;    // [batch][drafts + 1][vocab], [batch][drafts][vocab] or null
     const int32_t *draft_tokens, *counts;

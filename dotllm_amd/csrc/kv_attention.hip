@@ -717,7 +717,7 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
 constexpr int PRE_R = 2;
 constexpr int TARGET = 512;        // workgroups: two per CU
 constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (25.0 us against 27.6 at 512)
-constexpr size_t ARRIVED_BYTES = (size_t)4 * TARGET * COUNTER_STRIDE;   // entries * kv_heads <= TARGET where chunks are counted
+static_assert(TARGET <= MAX_SEQUENCES);   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
     Plan own{}, pre{};
@@ -765,8 +765,7 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
         x.o = reinterpret_cast<float*>(take(n * c.head_dim * 4));
         x.ml = reinterpret_cast<float*>(take(n * 8));
     };
-    // the counters come first in every workspace: what a call leaves there is zero for any other
-    o.arrived = reinterpret_cast<uint32_t*>(take(ARRIVED_BYTES));
+    o.arrived = reinterpret_cast<uint32_t*>(take(COUNTER_BYTES));
     if (prefix) {
         Plan& x = p.pre;
         x.rows = 16 * std::min(PRE_R, r);

@@ -47,7 +47,7 @@ struct SliceMass {
 };
 struct Work {              // in the workspace
     float* picked;         // [batch][rows] logit of each row's drafted token
-    uint32_t* drawn;       // [VERIFY_BATCH] workgroups done with a sequence, zero between launches
+    uint32_t* drawn;       // [MAX_SEQUENCES] workgroups done with a sequence, zero between launches
     SliceStats* stats;     // [batch][rows][slices], target rows first
     SliceMass* mass;       // [batch][slices]
     int rows, slices;
@@ -530,8 +530,7 @@ size_t layout(int batch, int drafts, int vocab, bool draft, uint8_t* base, Work*
         at += (n + 15) & ~(size_t)15;
         return p;
     };
-    // the counters come first in every workspace: what a call leaves there is zero for any other
-    w->drawn = reinterpret_cast<uint32_t*>(take((size_t)4 * VERIFY_BATCH * COUNTER_STRIDE));
+    w->drawn = reinterpret_cast<uint32_t*>(take(COUNTER_BYTES));
     w->picked = reinterpret_cast<float*>(take(sizeof(float) * (size_t)batch * w->rows));
     w->mass = reinterpret_cast<SliceMass*>(take(sizeof(SliceMass) * (size_t)batch * w->slices));
     w->stats = reinterpret_cast<SliceStats*>(take(sizeof(SliceStats) * (size_t)batch * w->rows * w->slices));

@@ -17,7 +17,8 @@
  *   - A workspace belongs to one call until that call's kernels have run: calls
  *     in the order of one stream may share it, graphs replayed at the same time
  *     may not.  It is zeroed once before its first call (llmdot_hip_device_alloc
- *     does that); every call leaves it fit for the next, whatever its sizes.
+ *     does that); every call leaves it fit for the next, whatever its sizes and
+ *     whichever of these operators it is for.
  *   - No counterpart in the reference, whose cache is fp32 and whose loop holds
  *     one sequence (src/Llmdot.Core/Inference/KvCache.cs).
  */
