@@ -347,12 +347,13 @@ __device__ __forceinline__ void join_weights(float& m, float mk, float& f, float
 }
 
 // Takes the 16 query rows from `first_row` on of a kv head (own rows: of sequence
-// b; a prefix's: of all sequences) for a tile: asks for the lane's part of them,
-// narrows the range of positions that all of them see, and returns where the
+// b; a prefix's: of all sequences, the lane's as `asked`) for a tile: asks for the
+// lane's part of them, narrows the range of positions that all of them see, and returns where the
 // lane's row goes in `out` (-1: none).
 template <int NB, bool PRE>
 __device__ __forceinline__ int64_t load_rows(const KvAttnArgs& a, Tile<NB>& t, f4 (&q)[2 * NB], int first_row, int b,
-                                             int head, const KvSpan& sp, int& edge_last, int& edge_before) {
+                                             int head, const KvSpan& sp, const KvAsked& asked, int& edge_last,
+                                             int& edge_before) {
     const int lane = threadIdx.x & 63, tokens = a.rows.tokens, group = (int)a.by_group.d;
     const int row = first_row + (lane & 15);
     int i, bb = b, token;
@@ -363,7 +364,7 @@ __device__ __forceinline__ int64_t load_rows(const KvAttnArgs& a, Tile<NB>& t, f
         bb = a.by_tokens.div(token);
         i = a.by_tokens.mod(token, bb);
         there = bb < a.rows.batch;
-        if (there) s = kv_span(a.rows, a.cache, bb);
+        s = kv_span(a.rows, a.cache, asked);
     } else {
         token = i = a.by_group.div(row);
         there = i < tokens;
@@ -456,10 +457,18 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
             v.load(vb + rec * VREC, lane);
         }
     };
-    // A prefix's rows are known only once their sequences' lengths are there: its
-    // record goes first.  Loads come back in order, so an own chunk asks for its
-    // queries, which are needed first, before its record.
-    if constexpr (PRE) load_record();
+    // A prefix's rows are known only once their sequences' lengths are there: their
+    // lengths, its record, then the queries.  Loads come back in order, so an own
+    // chunk asks for its queries, which are needed first, before its record.
+    KvAsked asked[R];
+    if constexpr (PRE) {
+#pragma unroll
+        for (int x = 0; x < R; x++) {
+            const int seq = a.by_tokens.div(a.by_group.div(tile * ROWS + x * 16 + (lane & 15)));
+            asked[x] = kv_asked(a.rows, seq < a.rows.batch ? seq : 0);
+        }
+        load_record();
+    }
     Tile<NB> t[R];
     int64_t out_at[R];     // element of `out` (-1: not a row)
     int edge_last = 0x7fffffff, edge_before = -1;   // records inside need no mask
@@ -468,7 +477,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         f4 q[R][2 * NB];
 #pragma unroll
         for (int x = 0; x < R; x++)
-            out_at[x] = load_rows<NB, PRE>(a, t[x], q[x], tile * ROWS + x * 16, b, head, sp, edge_last, edge_before);
+            out_at[x] = load_rows<NB, PRE>(a, t[x], q[x], tile * ROWS + x * 16, b, head, sp, asked[x], edge_last, edge_before);
         if constexpr (!PRE) load_record();
 #pragma unroll
         for (int x = 0; x < R; x++) {
@@ -664,7 +673,30 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     const int x = a.by_group.div(blockIdx.x), hr = a.by_group.mod(blockIdx.x, x), token = a.by_kv_heads.div(x),
               head = a.by_kv_heads.mod(x, token), h = head * group + hr;
     const int b = a.by_tokens.div(token), i = a.by_tokens.mod(token, b);
-    const KvSpan sp = kv_span(a.rows, a.cache, b);
+    const KvAsked asked = kv_asked(a.rows, b);
+
+    const int lanes = hd / 4, sets = THREADS / lanes;
+    const int set = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
+    float m = -INFINITY, l = 0.f;
+    f4 acc{0.f, 0.f, 0.f, 0.f};
+    auto take = [&](f2 ml, f4 o) {
+        float f, w;
+        join_weights(m, ml[0], f, w);
+        l = fmaf(l, f, w * ml[1]);
+        acc = acc * f + o * w;
+    };
+    // a set's chunks: of the prefix (whose place needs no lengths: the first is on
+    // its way while they come), then the row's own
+    const int prow = token * group + hr;
+    const int pchunks = pre.items ? pre.items / pre.entries : 0, ptile = pre.items ? prow / pre.rows : 0;
+    auto pre_part = [&](int k) { return ((int64_t)(ptile * pchunks + k) * kvh + head) * pre.rows + prow % pre.rows; };
+    f2 ml0{-INFINITY, 0.f};
+    f4 o0{0.f, 0.f, 0.f, 0.f};
+    if (set < sets && set < pchunks) {
+        ml0 = *reinterpret_cast<const f2*>(pre.ml + pre_part(set) * 2);
+        o0 = *reinterpret_cast<const f4*>(pre.o + pre_part(set) * hd + d);
+    }
+    const KvSpan sp = kv_span(a.rows, a.cache, asked);
     if (i < sp.lo || i >= sp.hi) return;
     const int row = i * group + hr, tile = row / own.rows, trow = row % own.rows;
     Cut c{0, 0, 1, 0, 0, sp};
@@ -673,26 +705,15 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     } else {
         c.first = b * own.tiles + tile;
     }
-    const int prow = token * group + hr;
-    const int pchunks = pre.items ? pre.items / pre.entries : 0, ptile = pre.items ? prow / pre.rows : 0;
     const int n = pchunks + c.count;
-
-    const int lanes = hd / 4, sets = THREADS / lanes;
-    const int set = threadIdx.x / lanes, d = threadIdx.x % lanes * 4;
-    float m = -INFINITY, l = 0.f;
-    f4 acc{0.f, 0.f, 0.f, 0.f};
     if (set < sets) {
+        if (set < pchunks) take(ml0, o0);
 #pragma unroll 4
-        for (int k = set; k < n; k += sets) {
+        for (int k = set < pchunks ? set + sets : set; k < n; k += sets) {
             const bool of_pre = k < pchunks;
-            const int64_t part = of_pre ? ((int64_t)(ptile * pchunks + k) * kvh + head) * pre.rows + prow % pre.rows
-                                        : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
-            const f2 ml = *reinterpret_cast<const f2*>((of_pre ? pre.ml : own.ml) + part * 2);
-            const f4 o = *reinterpret_cast<const f4*>((of_pre ? pre.o : own.o) + part * hd + d);
-            float f, w;
-            join_weights(m, ml[0], f, w);
-            l = fmaf(l, f, w * ml[1]);
-            acc = acc * f + o * w;
+            const int64_t part = of_pre ? pre_part(k) : ((int64_t)(c.first + k - pchunks) * kvh + head) * own.rows + trow;
+            take(*reinterpret_cast<const f2*>((of_pre ? pre.ml : own.ml) + part * 2),
+                 *reinterpret_cast<const f4*>((of_pre ? pre.o : own.o) + part * hd + d));
         }
     }
     __shared__ float so[THREADS * 4], sml[THREADS / 16][2];

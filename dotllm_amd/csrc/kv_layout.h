@@ -82,8 +82,12 @@ struct KvRows {                 // llmdot_hip_token_batch
 struct KvSpan {
     int slot, start, lo, hi;
 };
-__device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, int b) {
-    KvSpan s{r.slots[b], r.starts[b], 0, r.counts ? r.counts[b] : r.tokens};
+struct KvAsked { int slot, start, count; };   // a sequence as the arrays have it
+__device__ __forceinline__ KvAsked kv_asked(const KvRows& r, int b) {
+    return {r.slots[b], r.starts[b], r.counts ? r.counts[b] : r.tokens};
+}
+__device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, KvAsked a) {
+    KvSpan s{a.slot, a.start, 0, a.count};
     if (s.hi > r.tokens) s.hi = r.tokens;
     if (s.slot < 0 || s.slot >= c.slots || s.hi <= 0 || s.start >= c.capacity || s.start <= -r.tokens) {
         s.slot = s.start = s.hi = 0;
@@ -93,6 +97,9 @@ __device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, int 
     if (s.hi > c.capacity - s.start) s.hi = c.capacity - s.start;   // start > -2^31 here: no overflow
     if (s.hi < s.lo) s.hi = s.lo;
     return s;
+}
+__device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, int b) {
+    return kv_span(r, c, kv_asked(r, b));
 }
 
 }  // namespace llmdot
