@@ -278,15 +278,19 @@ __device__ __forceinline__ int wave_scan_int(int v) {
 // memory: one ratio of chunks to records for the whole batch, as high as the
 // items allow, so that long sequences get many workgroups and short ones few.
 // An entry of n records gets floor(n ratio) + 1 chunks: with ratio a little
-// under (items - entries) / records, all of them fit into the items.
+// under (items - entries) / records, all of them fit into the items; where the
+// lengths are such that they fit, it is (items - entries / 2) / records or
+// (items - 3 entries / 4) / records, and the longest chunk is that much shorter.
 __device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int item, bool by_entry) {
-    const float spare = (float)(pl.items - pl.entries) * (1.f - 0x1p-18f);
+    auto ratio_at = [&](float give, float records) {
+        return fminf(pl.per_record, ((float)pl.items - give * (float)pl.entries) * __builtin_amdgcn_rcpf(records));
+    };
     auto chunks = [&](float ratio, int n) { return n > 0 ? (int)((float)n * ratio) + 1 : 0; };
     if (pl.entries == 1) {
         const KvSpan sp = kv_span(a.rows, a.cache, 0);
         const int2 r = own_records(a, pl, sp, 0);
         const int n = r.y - r.x;
-        const int count = chunks(fminf(pl.per_record, spare * __builtin_amdgcn_rcpf((float)n)), n);
+        const int count = chunks(ratio_at(0.5f, (float)n), n);
         return Cut{by_entry || item < count ? 0 : -1, 0, count, r.x, r.y, sp};
     }
     const int lane = threadIdx.x & 63;
@@ -306,7 +310,14 @@ __device__ __forceinline__ Cut find_cut(const KvAttnArgs& a, const Plan& pl, int
         look(e0 + lane);
         total += (float)wave_sum_u32((uint32_t)(r.y - r.x));   // at most 64 * 2^25
     }
-    const float ratio = fminf(pl.per_record, spare * __builtin_amdgcn_rcpf(total));
+    float ratio = ratio_at(1.f, total) * (1.f - 0x1p-18f);
+    if (pl.entries <= 64) {
+#pragma unroll
+        for (float give : {0.75f, 0.5f}) {
+            const float more = ratio_at(give, total);
+            if (wave_sum_u32((uint32_t)chunks(more, r.y - r.x)) <= (uint32_t)pl.items) ratio = more;
+        }
+    }
     int before = 0;
     for (int e0 = 0; e0 < pl.entries; e0 += 64) {
         const int e = e0 + lane;
@@ -497,7 +508,9 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
             h8 kf[2][NB];
 #pragma unroll
             for (int i = 0; i < NB; i++) { kf[0][i] = k.q[i].k(0); kf[1][i] = k.q[i].k(1); }
+            if constexpr (FUSE) __builtin_amdgcn_s_setprio(1);
             scores<NB, R>(t, kf, k.d, v.e, s);
+            if constexpr (FUSE) __builtin_amdgcn_s_setprio(0);
         }
         k.load(kb + next * KREC, lane);
         if (rec * KV_GROUP + KV_GROUP - 1 > edge_last || rec * KV_GROUP <= edge_before) {
@@ -507,6 +520,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         h8 ph[R], pl8[R];
 #pragma unroll
         for (int x = 0; x < R; x++) t[x].probabilities(s[x], v.w, ph[x], pl8[x]);
+        if constexpr (FUSE) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < NB; i++) {
             const h8 d = v.d[i] * v.w;
@@ -521,6 +535,7 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
                 t[x].o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, lo, t[x].o[2 * i + 1], 0, 0, 0);
             }
         }
+        if constexpr (FUSE) __builtin_amdgcn_s_setprio(0);
         v.load(vb + next * VREC, lane);
     }
 #pragma unroll

@@ -84,19 +84,19 @@ struct KvSpan {
 };
 struct KvAsked { int slot, start, count; };   // a sequence as the arrays have it
 __device__ __forceinline__ KvAsked kv_asked(const KvRows& r, int b) {
-    return {r.slots[b], r.starts[b], r.counts ? r.counts[b] : r.tokens};
+    const int32_t* counts = r.counts ? r.counts : r.starts;   // no branch around a load
+    const int count = counts[b];
+    return {r.slots[b], r.starts[b], r.counts ? count : r.tokens};
 }
+// Selects, not branches: with an early way out the compiler asks for the three
+// numbers one after the other, each a trip to HBM.  Unsigned sums wrap where a
+// start is far outside, and are not used then.
 __device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, KvAsked a) {
-    KvSpan s{a.slot, a.start, 0, a.count};
-    if (s.hi > r.tokens) s.hi = r.tokens;
-    if (s.slot < 0 || s.slot >= c.slots || s.hi <= 0 || s.start >= c.capacity || s.start <= -r.tokens) {
-        s.slot = s.start = s.hi = 0;
-        return s;
-    }
-    if (s.start < 0) s.lo = -s.start;
-    if (s.hi > c.capacity - s.start) s.hi = c.capacity - s.start;   // start > -2^31 here: no overflow
-    if (s.hi < s.lo) s.hi = s.lo;
-    return s;
+    const int n = a.count < r.tokens ? a.count : r.tokens;
+    const bool there = (a.slot >= 0) & (a.slot < c.slots) & (n > 0) & (a.start < c.capacity) & (a.start > -r.tokens);
+    const int back = (int)(0u - (uint32_t)a.start), room = (int)((uint32_t)c.capacity - (uint32_t)a.start);
+    const int lo = back > 0 ? back : 0, most = n < room ? n : room, hi = most > lo ? most : lo;
+    return {there ? a.slot : 0, there ? a.start : 0, there ? lo : 0, there ? hi : 0};
 }
 __device__ __forceinline__ KvSpan kv_span(const KvRows& r, const KvView& c, int b) {
     return kv_span(r, c, kv_asked(r, b));
