@@ -15,6 +15,16 @@
 //     and dv 2^-e are halves, and ph dvn = hi + r exactly (r an fma), so
 //     P' = hi + (pl dvn + r) costs three packed instructions for two values.
 // Scores, statistics and sums are fp32.
+//
+// Bound by the issue of vector instructions for prompts (the MFMAs, 2 x 2 of 16
+// rows x 32 keys x 32 dims a block, run under them for the most part); by the
+// chain lengths -> queries and records -> joined wavefronts -> joined chunks for
+// single tokens.  Measured on an MI355X, whole calls:
+//   8 kv heads x 4 x 128, Q8_0: one token at 4096 positions 9.0 us; a prompt of
+//   2048 tokens 107 us (320 TFLOP/s of 4 hd per visible pair); 32 sequences of up
+//   to 250 positions behind 6000 shared ones 22 us.
+//   8 x 4 x 64, Q8_0 and Q4_0: 16 sequences of up to 8000 positions 16.7 us (2.9 TB/s).
+//   32 x 1 x 96, Q8_0: 4 x 5 drafted tokens at up to 2400 positions, window 2047, 11.1 us.
 #include "kernels.h"
 #include "kv_layout.h"
 
@@ -412,7 +422,9 @@ __device__ __forceinline__ int64_t load_rows(const KvAttnArgs& a, Tile<NB>& t, f
 // fourth of them to a wavefront.  Bound by instruction issue (about 200 vector
 // instructions a record and tile at head_dim 64, 300 at 128), by the loads'
 // latency where a wavefront has a record or two.  FUSE: the workgroup that
-// finishes an entry's last chunk joins them.
+// finishes an entry's last chunk joins them; its wavefronts' products go before
+// their neighbours' other work (16 long sequences of the 1B shape: 16.7 us, 17.5 without: two wavefronts of a SIMD drift
+// apart, and one's MFMAs run under the other's vector instructions).
 template <int NB, bool KQ4, bool VQ4, int R, bool PRE, bool FUSE>
 __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl, int wg, float* lds) {
     constexpr int HD = NB * 32, ROWS = 16 * R;
@@ -751,8 +763,8 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
 
 // ---- host ----
 constexpr int PRE_R = 2;
-constexpr int TARGET = 512;        // workgroups: two per CU
-constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (25.0 us against 27.6 at 512)
+constexpr int TARGET = 512;        // workgroups: two per CU (16 long sequences of the 1B shape: 16.7 us, 23.5 with 256)
+constexpr int PRE_TARGET = 256;    // of a prefix: its chunks' results cost more than an idle wavefront (22.1 us against 25.2 at 512)
 static_assert(TARGET <= MAX_SEQUENCES);   // entries * kv_heads <= TARGET where chunks are counted
 
 struct Plans {
@@ -767,7 +779,8 @@ int rows_per_wave(int blocks) { return blocks == 8 ? 1 : 2; }   // tiles of 16: 
 // Shapes of the launch, from sizes that the host knows (lengths are on the
 // device).  16 rows or fewer of a kv head and sequence (decode): tiles of 16
 // rows, more: of 32 (16 at head_dim 256, whose tiles leave no registers for
-// two wavefronts per SIMD).  A tile's keys go over the wavefronts of its
+// two wavefronts per SIMD): a record's integers become halves once for two tiles
+// (a 7B prompt of 2048 tokens: 107 us, 132 in tiles of 16).  A tile's keys go over the wavefronts of its
 // workgroup and, where tiles are too few for the card, in chunks over several.
 Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len, uint8_t* work) {
     Plans p;
@@ -779,7 +792,7 @@ Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix,
     o.rows = 16 * p.r;
     o.tiles = tiles_of(rows, o.rows);
     o.entries = batch * o.tiles;
-    // two records a wavefront pay for a chunk's own time (4096 keys of the 7B shape: 10.0 us, at one 11.7)
+    // two records a wavefront pay for a chunk's own time (4096 keys of the 7B shape: 9.0 us, at one 9.2, at four 10.9)
     o.least = 2 * WAVES;
     o.per_record = 1.f / (float)o.least * (1.f - 0x1p-18f);
     o.by_tiles = Divisor(o.tiles);

@@ -13,7 +13,9 @@
 // rows); then every workgroup decides its sequence's drafts for itself and sums
 // the residual in its slice of the one row that matters, and the last of them
 // finds the slice that holds the draw and scans it.  Bound by reading the logits
-// and, about as long, by the 64-bit exponentials.
+// and, about as long, by the 64-bit exponentials: 16 sequences of 5 drafts, 128256
+// logits and a draft model take 33.8 us (statistics 18, draw 17; 53 MB), one of 4
+// drafts and 32000 logits 10.5 (3 + 8: latencies).
 #include "kernels.h"
 #include "common.h"
 
@@ -517,7 +519,9 @@ __global__ __launch_bounds__(VT) void verify_draw(VerifyArgs a, Work w) {
     write_tokens(a, b, v.accepted, next);
 }
 
-// Logits of a slice: small ones where there are few slices to a row anyway.
+// Logits of a slice: small ones where there are few slices to a row anyway (one
+// sequence, vocabulary 32000: 10.5 us, 14.7 in slices of 4096), else large ones,
+// whose statistics every workgroup reads again (16 of 128256: 33.8, 50 of 1024).
 int quads_of(int vocab) { return vocab <= 32768 ? 1 : 4; }
 
 size_t layout(int batch, int drafts, int vocab, bool draft, uint8_t* base, Work* w) {
