@@ -23,7 +23,7 @@ import numpy as np
 from . import _lib
 from ._lib import call as _call
 from ._lib import lib, ptr
-from .device import DeviceArray, address
+from .device import DeviceArray, address, workspace_room
 
 def _f32(a, name: str) -> np.ndarray:
     if not (isinstance(a, np.ndarray) and a.dtype == np.float32 and a.flags["C_CONTIGUOUS"]):
@@ -242,8 +242,8 @@ class HipBackend:
         ap = address(accepted_out, "accepted_out", "int32", (b,), dev)
         qp = address(draft, "draft", "float32", (b, n, vocab), dev) if draft is not None else None
         cp = address(counts, "counts", "int32", (b,), dev) if counts is not None else None
-        _call(lib().llmdot_hip_verify_drafts(self._ctx, tp, qp, dp, cp, up, b, n, vocab, temperature, op, ap,
-                                             workspace.data_ptr(), workspace.nbytes))
+        wp, room = workspace_room(workspace, dev)
+        _call(lib().llmdot_hip_verify_drafts(self._ctx, tp, qp, dp, cp, up, b, n, vocab, temperature, op, ap, wp, room))
 
     # Members the LLaMA-like decode path does not call (other templates), on
     # the device like the rest (ICB:12, 18, 19, 25, 26).

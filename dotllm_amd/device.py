@@ -26,6 +26,8 @@ class DeviceArray:
         self.backend = backend
         self.shape = tuple(int(n) for n in (shape if hasattr(shape, "__len__") else (shape,)))
         self.dtype = np.dtype(dtype)
+        if any(n < 0 for n in self.shape):
+            raise ValueError(f"negative size in {self.shape}")
         self.size = int(np.prod(self.shape, dtype=np.int64))
         self.nbytes = self.size * self.dtype.itemsize
         self._p = C.c_void_p()
@@ -119,6 +121,15 @@ def _refuse(a, name: str, dtype: str, shape: tuple, device: int) -> None:
     raise ValueError(f"{name} must be contiguous")
 
 
+def workspace_room(a, device: int) -> tuple:
+    """Address and bytes of a workspace."""
+    if a.device.index != device:
+        raise ValueError(f"the workspace is on {a.device}, not on device {device}")
+    if not a.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
+    return a.data_ptr(), a.nbytes
+
+
 def rows(a, name: str, shape: tuple, device: int) -> tuple:
     """Address and row stride (floats) of a float32 array [batch, tokens, heads, head_dim] whose
     rows are whole and equally far apart: contiguous, or a slice of wider rows (a fused projection's)."""
@@ -132,6 +143,6 @@ def rows(a, name: str, shape: tuple, device: int) -> tuple:
     if 0 in shape or sd != 1 or (h > 1 and sh != d):
         raise ValueError(f"{name}'s rows must be contiguous")
     step = st if t > 1 else sb if b > 1 else 0
-    if b > 1 and t > 1 and sb != t * st:
+    if b > 1 and t > 1 and sb != t * st or b * t > 1 and step <= 0:   # the same row again: 0 would say packed
         raise ValueError(f"{name}'s rows must be equally far apart")
     return a.data_ptr(), step

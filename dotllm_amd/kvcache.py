@@ -21,14 +21,14 @@ import ctypes as C
 from . import _lib
 from ._lib import Q8_0, call, lib
 from .backend import HipBackend
-from .device import DeviceArray, address, rows
+from .device import DeviceArray, address, rows, workspace_room
 
 
 class TokenBatch:
     """The tokens of a call (:meth:`KvCache.batch`); keeps its arrays alive."""
 
-    def __init__(self, sequences: int, tokens: int, arrays: tuple, addresses: tuple):
-        self.sequences, self.tokens, self._arrays = sequences, tokens, arrays
+    def __init__(self, sequences: int, tokens: int, arrays: tuple, addresses: tuple, device: int):
+        self.sequences, self.tokens, self._arrays, self.device = sequences, tokens, arrays, device
         self.struct = _lib.TokenBatch(sequences, tokens, *addresses)
         self.ref = C.byref(self.struct)
 
@@ -77,20 +77,26 @@ class KvCache:
         dev = self.backend.device
         arrays = (slots, starts) + (() if counts is None else (counts,))
         at = [address(a, name, "int32", (n,), dev) for a, name in zip(arrays, ("slots", "starts", "counts"))]
-        return TokenBatch(n, int(tokens), arrays, (*at, *([None] * (3 - len(at)))))
+        return TokenBatch(n, int(tokens), arrays, (*at, *([None] * (3 - len(at)))), dev)
+
+    def _device(self, batch: TokenBatch) -> int:
+        dev = self.backend.device
+        if batch.device != dev:
+            raise ValueError(f"the batch is on device {batch.device}, the cache on device {dev}")
+        return dev
 
     def write(self, k, v, batch: TokenBatch) -> None:
         """Quantises k and v [sequences, tokens, kv_heads, head_dim] into the cache."""
-        shape = (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
-        kp, ks = rows(k, "k", shape, self.backend.device)
-        vp, vs = rows(v, "v", shape, self.backend.device)
+        dev, shape = self._device(batch), (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
+        kp, ks = rows(k, "k", shape, dev)
+        vp, vs = rows(v, "v", shape, dev)
         call(self._lib.llmdot_hip_kv_cache_write(self.handle, kp, ks, vp, vs, batch.ref))
 
     def read(self, k_out, v_out, batch: TokenBatch) -> None:
         """What the cache holds at the batch's positions, as fp32; other rows stay as they are."""
-        shape = (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
-        kp, ks = rows(k_out, "k_out", shape, self.backend.device)
-        vp, vs = rows(v_out, "v_out", shape, self.backend.device)
+        dev, shape = self._device(batch), (batch.sequences, batch.tokens, self.kv_heads, self.head_dim)
+        kp, ks = rows(k_out, "k_out", shape, dev)
+        vp, vs = rows(v_out, "v_out", shape, dev)
         call(self._lib.llmdot_hip_kv_cache_read(self.handle, kp, ks, vp, vs, batch.ref))
 
     def attention_workspace(self, heads: int, sequences: int, tokens: int, prefix: bool = False) -> DeviceArray:
@@ -106,10 +112,11 @@ class KvCache:
         [sequences, tokens, heads, head_dim].  Rows 0 .. prefix_len - 1 of slot `prefix_slot` of
         `prefix` come before every sequence's own; window > 0 keeps the last `window` positions;
         scale 0 is 1 / sqrt(head_dim).  Rows past a sequence's count stay as they are."""
+        dev = self._device(batch)
         shape = (batch.sequences, batch.tokens, q.shape[2] if len(q.shape) == 4 else 0, self.head_dim)
-        qp, qs = rows(q, "q", shape, self.backend.device)
-        op, os_ = rows(out, "out", shape, self.backend.device)
+        qp, qs = rows(q, "q", shape, dev)
+        op, os_ = rows(out, "out", shape, dev)
+        wp, room = workspace_room(workspace, dev)
         opt = _lib.Attention(shape[2], window, scale, prefix.handle if prefix is not None else None, prefix_slot,
                              prefix_len, qs, os_)
-        call(self._lib.llmdot_hip_kv_cache_attention(self.handle, qp, op, batch.ref, C.byref(opt), workspace.data_ptr(),
-                                                      workspace.nbytes))
+        call(self._lib.llmdot_hip_kv_cache_attention(self.handle, qp, op, batch.ref, C.byref(opt), wp, room))

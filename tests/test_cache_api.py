@@ -8,7 +8,8 @@ import numpy as np
 import pytest
 
 from dotllm_amd import _lib
-from dotllm_amd.device import address, rows
+from dotllm_amd.device import address, rows, workspace_room
+from dotllm_amd.kvcache import KvCache, TokenBatch
 from tests.kv_reference import attend, held, verify
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -98,6 +99,32 @@ def test_rows():
     for x in bad:
         with pytest.raises(ValueError):
             rows(x, "k", shape, 0)
+
+
+def test_rows_that_are_one_row_again():
+    """Broadcast rows (stride 0) are no packed rows."""
+    for shape, strides in (((2, 3, 4, 64), (0, 0, 64, 1)), ((1, 3, 4, 64), (768, 0, 64, 1)), ((3, 1, 4, 64), (0, 256, 64, 1))):
+        with pytest.raises(ValueError):
+            rows(_Tensor(shape, strides), "k", shape, 0)
+    assert rows(_Tensor((1, 1, 4, 64), (0, 0, 64, 1)), "k", (1, 1, 4, 64), 0) == (4096, 0)
+
+
+def test_workspace_and_batch_of_another_device():
+    ok = _Tensor((64,), dtype="torch.uint8")
+    ok.nbytes = 64
+    assert workspace_room(ok, 0) == (4096, 64)
+    for bad in (_Tensor((64,), index=1), _Tensor((64,), device="cpu", index=None), _Tensor((64,), (2,))):
+        bad.nbytes = 64
+        with pytest.raises(ValueError):
+            workspace_room(bad, 0)
+    cache = object.__new__(KvCache)   # no device is needed for what is refused before the library
+    cache._c, cache.kv_heads, cache.head_dim = None, 4, 64
+    cache.backend = type("B", (), dict(device=1))()
+    x, batch = _Tensor((1, 1, 4, 64), index=1), TokenBatch(1, 1, (), (None, None, None), 0)
+    for call in (lambda: cache.write(x, x, batch), lambda: cache.read(x, x, batch),
+                 lambda: cache.attention(x, x, batch, workspace=ok)):
+        with pytest.raises(ValueError, match="batch is on device 0"):
+            call()
 
 
 def test_address_of_an_array_interface():
