@@ -36,7 +36,7 @@ struct SliceStats {
     int32_t arg;
 };
 // A sequence's decision: the row that the next token comes from.
-struct Verdict {
+struct Decision {
     double zp, zq;         // masses of its target and draft rows
     float mp, mq;          // and maxima
     int32_t accepted;
@@ -57,51 +57,82 @@ struct Work {              // in the workspace
 
 // exp((x - mx) / T) for the logits x of a row with maximum mx.  2^y with y =
 // (x - mx) log2(e) / T: the nearest integer goes into the exponent, the rest
-// (|f| <= 1/2) through the Taylor series of 2^f, 11 terms: 6e-15 of the value.
+// (|f| <= 1/2) through a polynomial of degree 10 whose largest relative error
+// there is the least (2.2e-16, by Remez's exchange; 2.8e-16 with these doubles).
 // Adding and taking off 1.5 * 2^52 rounds to the integer and leaves it in the
 // low word: no conversions, which take four times an FMA's time.  Logits under
 // 2^-1000 of the maximum, -infinity and NaN have no mass.
-struct Series {            // ln2^i / i!, kept in scalar registers: as operands an FMA takes them in place
-    double c[12];
+struct Series {            // kept in scalar registers: as operands an FMA takes them in place
+    double c[11];
     __device__ __forceinline__ Series() {
-        constexpr double k[12] = {1.0, 6.9314718055994531e-01, 2.4022650695910071e-01, 5.5504108664821580e-02,
-                                  9.6181291076284772e-03, 1.3333558146428443e-03, 1.5403530393381608e-04,
-                                  1.5252733804059841e-05, 1.3215486790144309e-06, 1.0178086009239699e-07,
-                                  7.0549116208011234e-09, 4.4455382718708116e-10};
+        constexpr double k[11] = {1.0, 6.9314718055994973e-01, 2.4022650695908768e-01, 5.5504108664458839e-02,
+                                  9.6181291080346207e-03, 1.3333558228560802e-03, 1.5403529961092289e-04,
+                                  1.5252658116891647e-05, 1.3215662854692098e-06, 1.0208537850876446e-07,
+                                  7.0372755249486504e-09};
 #pragma unroll
-        for (int i = 0; i < 12; i++) {
+        for (int i = 0; i < 11; i++) {
             c[i] = k[i];
             asm("" : "+s"(c[i]));   // a number like any other to the compiler
         }
     }
     __device__ __forceinline__ double exp2(double f) const {
-        double r = fma(c[11], f, c[10]);
+        double r = fma(c[10], f, c[9]);
 #pragma unroll
-        for (int i = 9; i >= 0; i--) r = fma(r, f, c[i]);
+        for (int i = 8; i >= 0; i--) r = fma(r, f, c[i]);
         return r;
     }
 };
+constexpr double BIG = 6755399441055744.0;
+// One such number, for any x up to mx: 0 for NaN, 1 for the maximum itself.
+__device__ __forceinline__ double mass_of(float x, float mx, const VerifyArgs& a, const Series& series) {
+    const double d = (double)x - (double)mx, t = fma(d, a.rate, BIG);
+    const uint64_t u = __builtin_bit_cast(uint64_t, series.exp2(fma(d, a.rate, BIG - t)));
+    const double v = __builtin_bit_cast(double, u + (__builtin_bit_cast(uint64_t, t) << 52));
+    return x == mx ? 1.0 : d * a.rate > -1000.0 ? v : 0.0;
+}
+// The masses of a slice's logits.
 struct Masses {
-    double c, shift;       // y = c x + shift
-    float least;
+    double c, m;           // y = c (x - m)
+    float least;           // logits above it have a mass
     // a maximum of +infinity: only the infinities pass `least`, and y is 0 for them
     __device__ __forceinline__ Masses(float mx, const VerifyArgs& a) {
         const bool infinite = mx == INFINITY, none = !(mx > -INFINITY);
-        const double m = infinite || none ? 0.0 : (double)mx;
+        m = infinite || none ? 0.0 : (double)mx;
         c = infinite ? 0.0 : a.rate;
-        shift = -m * a.rate;
-        least = none ? INFINITY : infinite ? 3.4028234663852886e38f : (float)(m - a.reach);
+        // where floats (or doubles) lie further apart than the masses reach, the maximum stays above
+        const float low = __double2float_rd(m - a.reach);
+        least = none ? INFINITY : infinite ? 3.4028234663852886e38f : low < mx ? low : below(mx);
     }
     __device__ __forceinline__ double of(float x, const Series& series) const {
-        constexpr double BIG = 6755399441055744.0;
-        const double y = fma((double)__builtin_amdgcn_fmed3f(x, least, 3.4028234663852886e38f), c, shift);
-        const double t = y + BIG;
-        const double r = series.exp2(y - (t - BIG));
-        const uint64_t u = __builtin_bit_cast(uint64_t, r);
-        const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, t);   // the integer, modulo 2^32
+        uint32_t k;
+        const uint64_t u = significand(x, series, k);
         const bool some = x > least;
         const uint32_t high = some ? (uint32_t)(u >> 32) + (k << 20) : 0, low = some ? (uint32_t)u : 0;
         return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+    }
+    // `of` for sums that hold the maximum's own mass of 1: logits without mass count
+    // 2^-1000 or less each.  For a finite maximum with `least` no further below it
+    // than an exponent reaches.
+    __device__ __forceinline__ bool steady(float mx) const {
+        return mx > -INFINITY && mx < INFINITY && ((double)least - m) * c > -1020.0;
+    }
+    __device__ __forceinline__ double beside(float x, const Series& series) const {
+        uint32_t k;
+        const uint64_t u = significand(x, series, k);
+        return __builtin_bit_cast(double, u + ((uint64_t)k << 52));
+    }
+
+private:
+    __device__ __forceinline__ static float below(float v) {   // the next float, v finite
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        return __builtin_bit_cast(float, v > 0.f ? u - 1 : v < 0.f ? u + 1 : 0x80000001u);
+    }
+    // 2^f as a double's bits, and the integer modulo 2^32; x = m gives f = 0 whatever c
+    __device__ __forceinline__ uint64_t significand(float x, const Series& series, uint32_t& k) const {
+        const double d = (double)__builtin_amdgcn_fmed3f(x, least, 3.4028234663852886e38f) - m;
+        const double t = fma(d, c, BIG);
+        k = (uint32_t)__builtin_bit_cast(uint64_t, t);
+        return __builtin_bit_cast(uint64_t, series.exp2(fma(d, c, BIG - t)));
     }
 };
 
@@ -211,13 +242,14 @@ __device__ __forceinline__ void join_slices(const VerifyArgs& a, const SliceStat
     z = 0.0;
     for (int k = lane16; k < slices; k += 16) {
         const SliceStats t = s[k];
-        const float m = fmaxf(mx, t.mx);
-        const Masses e(m, a);   // against the larger maximum
-        z = z * e.of(mx, series) + t.z * e.of(t.mx, series);
+        const bool more = t.mx > mx;   // against the larger maximum
+        const float m = more ? t.mx : mx;
+        const double f = mass_of(more ? mx : t.mx, m, a, series);
+        z = more ? z * f + t.z : z + t.z * f;
         mx = m;
     }
     const float m = max16(mx);
-    z = sum16_64(z * Masses(m, a).of(mx, series));
+    z = sum16_64(z * mass_of(mx, m, a, series));
     mx = m;
 }
 // The first of a row's maxima, from its slices.
@@ -243,9 +275,9 @@ __device__ __forceinline__ int join_first(const SliceStats* s, int slices, int l
 // behind the first that does not, by the whole workgroup: 16 lanes a draft.  All
 // loads are of known addresses, so they are out at once.
 template <bool GREEDY>
-__device__ __forceinline__ Verdict decide(const VerifyArgs& a, const Work& w, int b) {
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, const Work& w, int b) {
     __shared__ int fail;
-    __shared__ Verdict of_set[VT / 16];
+    __shared__ Decision of_set[VT / 16];
     const int set = threadIdx.x / 16, lane16 = threadIdx.x & 15, n = draft_count(a, b);
     if (threadIdx.x == 0) fail = n;
     __syncthreads();
@@ -259,7 +291,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& a, const Work& w, in
             const int t = drafted ? a.draft_tokens[(int64_t)b * a.drafts + i] : -1;
             const double u = (double)a.uniforms[(int64_t)b * (a.drafts + 1) + i];
             bool stands = t >= 0 && t < a.vocab;
-            Verdict v{0.0, 0.0, 0.f, 0.f, i, -1, 0, 0};
+            Decision v{0.0, 0.0, 0.f, 0.f, i, -1, 0, 0};
             if constexpr (GREEDY) {
                 v.one = join_first(stats + (int64_t)i * w.slices, w.slices, lane16);
                 stands = stands && v.one == t;
@@ -269,9 +301,9 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& a, const Work& w, in
                 double q = 1.0;
                 if (with_q) {
                     join_slices(a, stats + (int64_t)(a.drafts + 1 + i) * w.slices, w.slices, lane16, series, v.mq, v.zq);
-                    q = v.zq > 0.0 ? Masses(v.mq, a).of(yt, series) / v.zq : 0.0;
+                    q = v.zq > 0.0 ? mass_of(yt, v.mq, a, series) / v.zq : 0.0;
                 }
-                const double p = v.zp > 0.0 ? Masses(v.mp, a).of(xt, series) / v.zp : 0.0;
+                const double p = v.zp > 0.0 ? mass_of(xt, v.mp, a, series) / v.zp : 0.0;
                 stands = stands && u * q < p;
                 // after the last draft the next token is the target's alone
                 v.has_q = with_q && i < n && v.zq > 0.0;
@@ -284,7 +316,7 @@ __device__ __forceinline__ Verdict decide(const VerifyArgs& a, const Work& w, in
         }
         __syncthreads();
         const int acc = fail;   // the same for all threads: the next write waits for the barrier
-        const Verdict v = of_set[acc < i0 + VT / 16 ? acc - i0 : 0];
+        const Decision v = of_set[acc < i0 + VT / 16 ? acc - i0 : 0];
         __syncthreads();
         if (acc < i0 + VT / 16) return v;
     }
@@ -337,10 +369,17 @@ __global__ __launch_bounds__(VT) void verify_stats(VerifyArgs a, Work w) {
     } else {
         const Masses e(mx, a);
         const Series series;
+        if (e.steady(mx)) {
 #pragma unroll
-        for (int j = 0; j < Q; j++)
+            for (int j = 0; j < Q; j++)
 #pragma unroll
-            for (int k = 0; k < QUAD; k++) z += e.of(x[j][k], series);
+                for (int k = 0; k < QUAD; k++) z += e.beside(x[j][k], series);
+        } else {
+#pragma unroll
+            for (int j = 0; j < Q; j++)
+#pragma unroll
+                for (int k = 0; k < QUAD; k++) z += e.of(x[j][k], series);
+        }
         z = wave_sum64(z);
         if (lane == 0) sz[wave] = z;
         __syncthreads();
@@ -353,7 +392,7 @@ __global__ __launch_bounds__(VT) void verify_stats(VerifyArgs a, Work w) {
 
 __global__ __launch_bounds__(VT) void verify_greedy(VerifyArgs a, Work w) {
     const int b = blockIdx.x;
-    const Verdict v = decide<true>(a, w, b);
+    const Decision v = decide<true>(a, w, b);
     write_tokens(a, b, v.accepted, v.one);
 }
 
@@ -363,7 +402,7 @@ struct Residual {
     Masses p, q;
     double ip, iq;         // 1 / masses, 0 without any
     int one;
-    __device__ __forceinline__ Residual(const Verdict& v, const VerifyArgs& a)
+    __device__ __forceinline__ Residual(const Decision& v, const VerifyArgs& a)
         : p(v.mp, a), q(v.mq, a), ip(v.zp > 0.0 ? 1.0 / v.zp : 0.0), iq(v.has_q ? 1.0 / v.zq : 0.0), one(v.one) {}
     __device__ __forceinline__ double of(float x, float y, int t, double& pt) const {
         pt = p.of(x, series) * ip;
@@ -401,7 +440,7 @@ __global__ __launch_bounds__(VT) void verify_draw(VerifyArgs a, Work w) {
     __shared__ int next;
     const int slice = blockIdx.x % w.slices, b = blockIdx.x / w.slices;
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    Verdict v = decide<false>(a, w, b);
+    Decision v = decide<false>(a, w, b);
     const double u = (double)a.uniforms[(int64_t)b * (a.drafts + 1) + a.drafts];
     const float* target = target_row(a, b, v.accepted);
     const float* draft = v.has_q ? draft_row(a, b, v.accepted) : target;

@@ -84,13 +84,23 @@ class DeviceArray:
 
 
 _NAMES = {"float32": ("float32", "torch.float32"), "int32": ("int32", "torch.int32")}
+_KNOWN = {"float32": set(), "int32": set()}   # types of other libraries that go by these names
+
+
+def _typed(dtype, name: str) -> bool:
+    if dtype in _KNOWN[name]:
+        return True
+    if str(dtype) in _NAMES[name]:
+        _KNOWN[name].add(dtype)
+        return True
+    return False
 
 
 def address(a, name: str, dtype: str, shape: tuple, device: int) -> int:
     """The address of a contiguous device array of the given type and shape."""
     where = getattr(a, "data_ptr", None)
     if where is not None:
-        if a.device.index != device or a.shape != shape or str(a.dtype) not in _NAMES[dtype] or not a.is_contiguous():
+        if a.device.index != device or a.shape != shape or not _typed(a.dtype, dtype) or not a.is_contiguous():
             _refuse(a, name, dtype, shape, device)
         return where()
     face = getattr(a, "__cuda_array_interface__", None)
@@ -116,7 +126,7 @@ def _refuse(a, name: str, dtype: str, shape: tuple, device: int) -> None:
         raise ValueError(f"{name} is on {a.device}, not on device {device}")
     if tuple(a.shape) != shape:
         raise ValueError(f"{name} must have shape {shape}, not {tuple(a.shape)}")
-    if str(a.dtype) not in _NAMES[dtype]:
+    if not _typed(a.dtype, dtype):
         raise ValueError(f"{name} must be {dtype}, not {a.dtype}")
     raise ValueError(f"{name} must be contiguous")
 
@@ -134,10 +144,12 @@ def rows(a, name: str, shape: tuple, device: int) -> tuple:
     """Address and row stride (floats) of a float32 array [batch, tokens, heads, head_dim] whose
     rows are whole and equally far apart: contiguous, or a slice of wider rows (a fused projection's)."""
     stride = getattr(a, "stride", None)
-    if stride is None or a.is_contiguous():
+    if stride is None:
         return address(a, name, "float32", shape, device), 0
-    if a.device.index != device or a.shape != shape or str(a.dtype) not in _NAMES["float32"]:
+    if a.device.index != device or a.shape != shape or not (a.dtype in _KNOWN["float32"] or _typed(a.dtype, "float32")):
         _refuse(a, name, "float32", shape, device)
+    if a.is_contiguous():
+        return a.data_ptr(), 0
     b, t, h, d = shape
     sb, st, sh, sd = stride()
     if 0 in shape or sd != 1 or (h > 1 and sh != d):

@@ -155,3 +155,21 @@ def test_refusals(hip):
         hip.verify_workspace(1, 1, (1 << 24) + 1)
     with pytest.raises(ValueError):
         hip.verify_workspace(1, -1, 100)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e12, 1e30, 3e38])
+@pytest.mark.parametrize("temperature", [1e-30, 0.8, 1e20, 3e38])
+def test_far_apart(hip, size, temperature):
+    """Logits between which floats lie further apart than any mass reaches, temperatures at the ends of their range,
+    logits without mass among them."""
+    rng = np.random.default_rng(17)
+    target, draft, drafts, u = logits(rng, 4, 3, 1500)
+    for x in (target, draft):
+        x[:] = (x / np.abs(x).max() * size).astype(np.float32)
+        x[0, :, ::3] = -np.inf
+        x[1, :, ::2] = np.nan
+        x[2, :, :1499] = -np.inf
+    drafts[0] = target[0, :3].argmax(-1)
+    drafts[2] = 1499
+    check(hip, target, drafts, u, temperature, draft)
+    check(hip, target, drafts, u, temperature)
