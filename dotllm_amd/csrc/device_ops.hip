@@ -217,7 +217,7 @@ extern "C" int32_t llmdot_hip_kv_cache_attention(llmdot_hip_kv_cache* cache, con
         if (int rc = check_stride("q", width, &a.q_stride)) return rc;
         if (int rc = check_stride("out", width, &a.out_stride)) return rc;
         if (opt->window < 0) return ctx_fail(LLMDOT_E_INVALID, "negative window");
-        if (!(opt->scale >= 0.f) || opt->scale > 3e38f) return ctx_fail(LLMDOT_E_INVALID, "scale must be a number of at least 0");
+        if (!(opt->scale >= 0.f) || opt->scale > 2e38f) return ctx_fail(LLMDOT_E_INVALID, "scale must be a number of at least 0");
         if (opt->prefix_len < 0) return ctx_fail(LLMDOT_E_INVALID, "negative prefix length");
         if (opt->prefix_len > 0 && !opt->prefix) return ctx_fail(LLMDOT_E_INVALID, "a prefix length without a prefix");
         if (opt->prefix && opt->prefix_len > 0) {

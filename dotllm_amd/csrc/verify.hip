@@ -14,8 +14,8 @@
 // the residual in its slice of the one row that matters, and the last of them
 // finds the slice that holds the draw and scans it.  Bound by reading the logits
 // and, about as long, by the 64-bit exponentials: 16 sequences of 5 drafts, 128256
-// logits and a draft model take 33.8 us (statistics 18, draw 17; 53 MB), one of 4
-// drafts and 32000 logits 10.5 (3 + 8: latencies).
+// logits and a draft model take 32.5 us (statistics 17, draw 17; 53 MB), one of 4
+// drafts and 32000 logits 10.4 (3 + 8: latencies).
 #include "kernels.h"
 #include "common.h"
 
@@ -559,8 +559,8 @@ __global__ __launch_bounds__(VT) void verify_draw(VerifyArgs a, Work w) {
 }
 
 // Logits of a slice: small ones where there are few slices to a row anyway (one
-// sequence, vocabulary 32000: 10.5 us, 14.7 in slices of 4096), else large ones,
-// whose statistics every workgroup reads again (16 of 128256: 33.8, 50 of 1024).
+// sequence, vocabulary 32000: 10.4 us, 15.6 in slices of 4096), else large ones,
+// whose statistics every workgroup reads again (16 of 128256: 32.5, 49 of 1024).
 int quads_of(int vocab) { return vocab <= 32768 ? 1 : 4; }
 
 size_t layout(int batch, int drafts, int vocab, bool draft, uint8_t* base, Work* w) {

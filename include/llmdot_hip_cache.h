@@ -87,7 +87,7 @@ int32_t llmdot_hip_kv_cache_read(llmdot_hip_kv_cache* cache, float* k_dev, int64
 typedef struct llmdot_hip_attention {
     int32_t heads;               /* a multiple of kv_heads */
     int32_t window;              /* 0: every earlier position */
-    float scale;                 /* 0: 1 / sqrt(head_dim) */
+    float scale;                 /* 0: 1 / sqrt(head_dim); at most 2e38 */
     const llmdot_hip_kv_cache* prefix;   /* NULL: none */
     int32_t prefix_slot, prefix_len;
     int64_t q_stride, out_stride;        /* as above */
