@@ -512,6 +512,29 @@ __device__ __forceinline__ void attend_chunk(const KvAttnArgs& a, const Plan& pl
         }
     }
     if (PRE && edge_last > a.prefix_len - 1) edge_last = a.prefix_len - 1;
+    if (PRE && a.window > 0) {
+        // rows whose windows begin behind the chunk (a prompt's, all but the first few): nothing to join
+        int before = 0x7fffffff;
+#pragma unroll
+        for (int x = 0; x < R; x++)
+            if (out_at[x] >= 0 && t[x].before < before) before = t[x].before;
+#pragma unroll
+        for (int k = 1; k < 16; k *= 2) {
+            const int o = __shfl_xor(before, k);
+            before = o < before ? o : before;
+        }
+        const int end = r1 * KV_GROUP < a.prefix_len ? r1 * KV_GROUP : a.prefix_len;
+        if (__builtin_amdgcn_readfirstlane(before) >= end - 1) {
+            if (wave == 0 && g == 0) {
+#pragma unroll
+                for (int x = 0; x < R; x++) {
+                    const int64_t part = ((int64_t)at_item * kvh + head) * ROWS + x * 16 + (lane & 15);
+                    *reinterpret_cast<f2*>(pl.ml + part * 2) = f2{-INFINITY, 0.f};
+                }
+            }
+            return;
+        }
+    }
 
     for (; rec < r1; rec += WAVES) {
         const int next = rec + WAVES < r1 ? rec + WAVES : rec;
@@ -707,6 +730,7 @@ __global__ __launch_bounds__(THREADS) void kv_attention_join(KvAttnArgs a, Plan 
     float m = -INFINITY, l = 0.f;
     f4 acc{0.f, 0.f, 0.f, 0.f};
     auto take = [&](f2 ml, f4 o) {
+        if (ml[0] == -INFINITY) return;   // saw nothing: its sums may not have been written
         float f, w;
         join_weights(m, ml[0], f, w);
         l = fmaf(l, f, w * ml[1]);
@@ -785,7 +809,9 @@ int rows_per_wave(int blocks) { return blocks == 8 ? 1 : 2; }   // tiles of 16: 
 Plans make_plans(const KvView& c, int heads, int batch, int tokens, bool prefix, int prefix_len, uint8_t* work) {
     Plans p;
     const int group = heads / c.kv_heads, r = rows_per_wave(c.head_dim / 32);
-    const int64_t rows = (int64_t)tokens * group, want = TARGET / c.kv_heads;
+    // beside a prefix the call's own chunks get the other half of the workgroups (431 tokens of 2 heads at
+    // position 3234 behind 11433: 30 us, 36 with all of them, whose last then wait for a place)
+    const int64_t rows = (int64_t)tokens * group, want = (prefix ? TARGET - PRE_TARGET : TARGET) / c.kv_heads;
     auto tiles_of = [](int64_t n, int per) { return (int)((n + per - 1) / per); };
     p.r = rows <= 16 ? 1 : r;
     Plan& o = p.own;
@@ -866,7 +892,8 @@ bool kv_attention_supported(int head_dim) {
 }
 
 size_t kv_attention_workspace(const KvView& c, int heads, int batch, int tokens, bool prefix) {
-    return make_plans(c, heads, batch, tokens, prefix, -1, nullptr).bytes;
+    const size_t without = make_plans(c, heads, batch, tokens, false, 0, nullptr).bytes;
+    return prefix ? std::max(without, make_plans(c, heads, batch, tokens, true, -1, nullptr).bytes) : without;
 }
 
 size_t kv_attention_workspace_upto(const KvView& c, int heads, int tokens) {

@@ -266,3 +266,27 @@ def test_refusals(hip):
         cache.attention_workspace(3, 1, 1)
     with pytest.raises(ValueError):
         cache.attention_workspace(4, -1, 1)
+
+
+@pytest.mark.parametrize("head_dim,kv_heads,group", [(64, 2, 4), (128, 1, 2), (256, 2, 7)])
+@pytest.mark.parametrize("window", [1, 20, 32, 70])
+def test_prompt_that_leaves_its_prefix_behind(hip, head_dim, kv_heads, group, window):
+    """Windows that only the first rows of a prompt share with the prefix, in a workspace that holds NaN where parts
+    are not written."""
+    case = Case(hip, kv_heads, head_dim, [200, 131], prefix=90, capacity=200, seed=window)
+    ws = case.cache.attention_workspace(kv_heads * group, 2, 131, True)
+    fill = np.zeros(ws.nbytes, np.uint8)
+    fill[1 << 19:] = 255          # behind the counters
+    ws.put(fill)
+    case.cache.attention_workspace = lambda *a: ws
+    case.check(kv_heads * group, 131, [69, 0], [131, 100], window=window)
+    case.check(kv_heads * group, 131, [0, 0], [5, 131], window=window)
+
+
+def test_workspace_with_a_prefix_serves_calls_without(hip):
+    """Whatever the plan: the larger of the two."""
+    cache = KvCache(hip, 1, 1, 64, 4000)
+    for heads in (1, 2, 8):
+        for batch, tokens in ((1, 1), (1, 500), (1, 2065), (3, 700), (129, 1), (300, 5), (500, 1)):
+            assert (cache.attention_workspace(heads, batch, tokens, True).nbytes
+                    >= cache.attention_workspace(heads, batch, tokens).nbytes)
