@@ -270,7 +270,8 @@ __global__ __launch_bounds__(THREADS) void kv_read_kernel(KvView c, KvRows rows,
     }
 }
 
-// One wavefront per head row of a token (q heads, then k, then v).
+// One wavefront per head row of a token (q heads, then k, then v).  Bound by the
+// launch for a token, by reading and writing the rows for a prompt.
 __global__ __launch_bounds__(64) void rope_rows_kernel(PfAttnArgs a, const int32_t* start, float* q_out, float* k_out,
                                                        float* v_out) {
     const int hd = a.head_dim, t = blockIdx.x, lane = threadIdx.x, half = a.rope_half;
