@@ -21,7 +21,7 @@
 // chain lengths -> queries and records -> joined wavefronts -> joined chunks for
 // single tokens.  Measured on an MI355X, whole calls:
 //   8 kv heads x 4 x 128, Q8_0: one token at 4096 positions 9.0 us; a prompt of
-//   2048 tokens 107 us (320 TFLOP/s of 4 hd per visible pair); 32 sequences of up
+//   2048 tokens 106 to 109 us (320 TFLOP/s of 4 hd per visible pair); 32 sequences of up
 //   to 250 positions behind 6000 shared ones 22 us.
 //   8 x 4 x 64, Q8_0 and Q4_0: 16 sequences of up to 8000 positions 16.7 us (2.9 TB/s).
 //   32 x 1 x 96, Q8_0: 4 x 5 drafted tokens at up to 2400 positions, window 2047, 11.1 us.
